@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import os
 from pathlib import Path
+from typing import NamedTuple
 
 import torch
 
@@ -34,11 +35,20 @@ def build_extension(verbose: bool = False):
             name="baguanet_C",
             sources=[
                 str(src / "torch" / "ops.cc"),
+                str(src / "torch" / "train_ops.cc"),
                 str(src / "hip" / "pack_kernels.hip"),
                 str(src / "hip" / "multi_tensor.hip"),
+                str(src / "hip" / "embedding.hip"),
+                str(src / "hip" / "residual_norm.hip"),
+                str(src / "hip" / "act8.hip"),
+                str(src / "hip" / "act8_wgrad.hip"),
             ],
             build_directory=str(build_dir),
             extra_cflags=["-O3"],
+            # packed fp32 instructions stay out of every kernel: some of
+            # their forms have given wrong results on this hardware
+            extra_cuda_cflags=["-O3", "-Xclang", "-target-feature",
+                               "-Xclang", "-packed-fp32-ops"],
             verbose=verbose,
         )
     except Exception as e:  # pragma: no cover
@@ -70,3 +80,119 @@ def fused_sgd(params, grads, momenta, lr, momentum=0.0, weight_decay=0.0,
               nesterov=False) -> None:
     _load().fused_sgd(params, grads, momenta, lr, momentum, weight_decay,
                       nesterov)
+
+
+# ---------------------------------------------------------------------------
+# Training-step operators.  Each takes float32, bfloat16 or float16 tensors on
+# the GPU, runs on the current stream, sums in float32 and rounds once; each
+# is differentiable once, with the same result in every run.
+
+
+def embedding(weight: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
+              padding_idx: int | None = None,
+              out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``scale * weight[tokens]``, of the shape ``[*tokens.shape, dim]``.
+
+    ``weight`` is ``[vocab, dim]``, ``tokens`` int64 or int32 of any shape;
+    the result has ``out_dtype`` (default: the weight's type).  The weight's
+    gradient is dense, in the weight's type: each row is the sum over the
+    token's places, in their order, times ``scale``.  The row of
+    ``padding_idx`` takes no gradient.  A token outside the table gives a row
+    of NaN and no gradient.
+    """
+    return _load().embedding(weight, tokens, scale, padding_idx, out_dtype)
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
+             eps: float = 1e-6) -> torch.Tensor:
+    """``x / sqrt(mean(x ** 2) + eps) * weight`` over the last dimension.
+
+    ``weight`` is ``[dim]``, float32 or of x's type; ``dim`` is at most
+    32768.  This is the norm before a network's first block; those between
+    blocks are part of :func:`gated_residual_norm`.
+    """
+    return _load().rms_norm(x, weight, eps)
+
+
+def gated_residual_norm(x: torch.Tensor, branch: torch.Tensor,
+                        gate: torch.Tensor | None = None,
+                        post_weight: torch.Tensor | None = None,
+                        pre_weight: torch.Tensor | None = None,
+                        residual_scale: float = 1.0,
+                        branch_scale: float = 1.0, eps: float = 1e-6,
+                        ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """The seam between two blocks of a network, in one pass::
+
+        u = rms_norm(branch, post_weight)          (branch, without a weight)
+        y = residual_scale * x + branch_scale * gate * u
+        h = rms_norm(y, pre_weight)                (None, without a weight)
+
+    Returns ``(y, h)``: the residual stream and the next block's input.
+    ``x`` and ``branch`` have one shape and type, with at most 32768 columns.
+    ``gate`` may be anything that broadcasts to x: ``[dim]`` for each column,
+    ``[batch, 1, dim]`` for each sequence's columns, ``[batch, length, 1]``
+    for each row, or one value for each element.  It and the weights are
+    float32 or of x's type, and all of them take gradients.
+    """
+    return _load().gated_residual_norm(x, branch, gate, post_weight,
+                                       pre_weight, residual_scale,
+                                       branch_scale, eps)
+
+
+class Act8(NamedTuple):
+    """An activation kept in 8 bits (see :func:`act8_pack`)."""
+
+    codes: torch.Tensor
+    exponents: torch.Tensor
+    shape: torch.Size
+    dtype: torch.dtype
+
+
+def act8_pack(x: torch.Tensor) -> Act8:
+    """An 8-bit copy of ``x``, to keep from the forward to the backward pass.
+
+    Groups of 32 neighbours of a row share a power of two that brings the
+    largest to at most 448; each value is then an e4m3 number.  A value is
+    off by at most 1/16 of itself, or by 2**-19 of its group's largest if
+    that is more.  NaN and infinities are kept as NaN.  The copy takes 33
+    bytes for 32 values and no part in autograd.
+    """
+    codes, exponents = _load().act8_pack(x)
+    return Act8(codes, exponents, x.shape, x.dtype)
+
+
+def act8_unpack(kept: Act8) -> torch.Tensor:
+    """The values that an 8-bit copy stands for, exact in its type."""
+    return _load().act8_unpack(kept.codes, kept.exponents, list(kept.shape),
+                               kept.dtype)
+
+
+def act8_wgrad(dy: torch.Tensor, kept: Act8, bias: bool = True,
+               ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """A linear layer's weight gradient ``dy^T x`` from the 8-bit copy of x.
+
+    ``dy`` has the rows of ``kept`` and its type.  Returns ``(dw, db)``, with
+    ``db`` the sum of dy's rows, or None without ``bias``.
+    """
+    return _load().act8_wgrad(dy, kept.codes, kept.exponents,
+                              list(kept.shape), kept.dtype, bias)
+
+
+def linear_act8(x: torch.Tensor, weight: torch.Tensor,
+                bias: torch.Tensor | None = None) -> torch.Tensor:
+    """``torch.nn.functional.linear`` with its input kept in 8 bits.
+
+    The result and x's gradient are those of a linear layer; the weight's
+    gradient is :func:`act8_wgrad` of the 8-bit copy, which takes the place
+    of x in the memory that the graph holds.
+    """
+    return _load().linear_act8(x, weight, bias)
+
+
+def silu_mul_act8(x: torch.Tensor) -> torch.Tensor:
+    """``silu(a) * b`` for ``a, b = x.chunk(2, -1)``, kept in 8 bits.
+
+    The result is that of x itself; its gradient is taken at the 8-bit
+    copies of a and b, which are all that the graph holds.
+    """
+    return _load().silu_mul_act8(x)

@@ -1,0 +1,191 @@
+// act8.hip — activation checkpoints in 8 bits (gfx950).
+//
+// A group of 32 neighbouring values of a row is kept as q[i] * 2^e, q in
+// e4m3 (round to nearest even), with the smallest e that brings the largest
+// finite value to at most 448 = max(e4m3).  2^e is a power of two so that
+// q * 2^e is exact in the activation's own type: e is held to the range
+// where that is so, [-117, 120] for bf16 and fp32, [-15, 8] for fp16, and at
+// its upper end q stops at 240, the last value whose product stays finite.
+// A value is off by at most 1/16 of itself, or by 2^(e-10) below 2^(e-6).
+// A NaN or an infinity is kept as NaN and does not enter its group's scale.
+//
+// These kernels are bound by HBM; four lanes hold a group, 8 values each, and
+// find its largest value with two lane exchanges.
+#include <hip/hip_runtime.h>
+
+#include "act8_codes.h"
+
+namespace baguanet {
+namespace {
+
+constexpr int kBlock = 256;
+
+// `tpr` lanes (a power of two, 4 to kBlock) move one row.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void act8_pack_kernel(Act8Move a,
+                                                           int tpr) {
+  const int team = threadIdx.x / tpr, lane = threadIdx.x % tpr;
+  const int64_t teams = kBlock / tpr;
+  for (int64_t r = (int64_t)blockIdx.x * teams + team; r < a.rows;
+       r += (int64_t)gridDim.x * teams) {
+    const T* src = (const T*)a.x + r * a.xstride;
+    for (int64_t c = (int64_t)lane * kVec; c < a.pitch;
+         c += (int64_t)tpr * kVec) {
+      float8 v = 0.f;
+      if (c < a.cols)
+        v = load_upto(src + c, (int)(a.cols - c < kVec ? a.cols - c : kVec));
+      const int e = group_power<T>(v);
+      *(uint2*)(a.codes + r * a.pitch + c) = encode8<T>(v, e);
+      if (c % kAct8Group == 0)
+        a.exps[(r * a.pitch + c) / kAct8Group] = (uint8_t)(e + 127);
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kBlock) void act8_unpack_kernel(Act8Move a,
+                                                             int tpr) {
+  const int team = threadIdx.x / tpr, lane = threadIdx.x % tpr;
+  const int64_t teams = kBlock / tpr;
+  for (int64_t r = (int64_t)blockIdx.x * teams + team; r < a.rows;
+       r += (int64_t)gridDim.x * teams) {
+    T* dst = (T*)a.x + r * a.xstride;
+    for (int64_t c = (int64_t)lane * kVec; c < a.cols;
+         c += (int64_t)tpr * kVec) {
+      const uint2 q = *(const uint2*)(a.codes + r * a.pitch + c);
+      const int e = a.exps[(r * a.pitch + c) / kAct8Group] - 127;
+      store_upto(dst + c, decode8(q, e),
+                 (int)(a.cols - c < kVec ? a.cols - c : kVec));
+    }
+  }
+}
+
+// ---- out = silu(a) * b, its inputs kept in 8 bits --------------------------
+// x holds a in its first `cols` columns and b in the others.  With the kept
+// values a', b' and s = 1 / (1 + exp(-a')):
+//   da = dout * b' * s * (1 + a' * (1 - s))     db = dout * a' * s
+
+__device__ inline float sigmoid(float a) {
+  return __builtin_amdgcn_rcpf(1.f + expf(-a));
+}
+
+template <typename T>
+__global__ __launch_bounds__(kBlock) void silu_forward_kernel(SiluAct8 p,
+                                                              int tpr) {
+  const int team = threadIdx.x / tpr, lane = threadIdx.x % tpr;
+  const int64_t teams = kBlock / tpr;
+  for (int64_t r = (int64_t)blockIdx.x * teams + team; r < p.rows;
+       r += (int64_t)gridDim.x * teams) {
+    const T* src = (const T*)p.x + r * p.xstride;
+    for (int64_t c = (int64_t)lane * kVec; c < p.pitch;
+         c += (int64_t)tpr * kVec) {
+      float8 a = 0.f, b = 0.f, o;
+      const int m = c < p.cols ? (int)(p.cols - c < kVec ? p.cols - c : kVec)
+                               : 0;
+      if (m) {
+        a = load_upto(src + c, m);
+        b = load_upto(src + p.cols + c, m);
+#pragma unroll
+        for (int i = 0; i < kVec; i++) o[i] = a[i] * sigmoid(a[i]) * b[i];
+        store_upto((T*)p.out + r * p.cols + c, o, m);
+      }
+      if (!p.codes) continue;
+      const int ea = group_power<T>(a), eb = group_power<T>(b);
+      uint8_t* q = p.codes + r * 2 * p.pitch + c;
+      *(uint2*)q = encode8<T>(a, ea);
+      *(uint2*)(q + p.pitch) = encode8<T>(b, eb);
+      if (c % kAct8Group == 0) {
+        uint8_t* e = p.exps + (r * 2 * p.pitch + c) / kAct8Group;
+        e[0] = (uint8_t)(ea + 127);
+        e[p.pitch / kAct8Group] = (uint8_t)(eb + 127);
+      }
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kBlock) void silu_backward_kernel(SiluAct8 p,
+                                                               int tpr) {
+  const int team = threadIdx.x / tpr, lane = threadIdx.x % tpr;
+  const int64_t teams = kBlock / tpr;
+  for (int64_t r = (int64_t)blockIdx.x * teams + team; r < p.rows;
+       r += (int64_t)gridDim.x * teams) {
+    for (int64_t c = (int64_t)lane * kVec; c < p.cols;
+         c += (int64_t)tpr * kVec) {
+      const int m = (int)(p.cols - c < kVec ? p.cols - c : kVec);
+      const uint8_t* q = p.codes + r * 2 * p.pitch + c;
+      const uint8_t* e = p.exps + (r * 2 * p.pitch + c) / kAct8Group;
+      const float8 a = decode8(*(const uint2*)q, e[0] - 127);
+      const float8 b = decode8(*(const uint2*)(q + p.pitch),
+                               e[p.pitch / kAct8Group] - 127);
+      const float8 d =
+          load_upto((const T*)p.dout + r * p.dstride + c, m);
+      float8 da, db;
+#pragma unroll
+      for (int i = 0; i < kVec; i++) {
+        const float s = sigmoid(a[i]);
+        da[i] = d[i] * b[i] * s * (1.f + a[i] * (1.f - s));
+        db[i] = d[i] * a[i] * s;
+      }
+      T* dst = (T*)p.dx + r * 2 * p.cols + c;
+      store_upto(dst, da, m);
+      store_upto(dst + p.cols, db, m);
+    }
+  }
+}
+
+int team_size(int64_t pitch) {
+  int tpr = kAct8Group / kVec;
+  while (tpr < kBlock && (int64_t)tpr * kVec < pitch) tpr *= 2;
+  return tpr;
+}
+
+// One team for each row, up to enough workgroups to fill the chip.
+uint32_t row_grid(int64_t rows, int tpr) {
+  const int64_t teams = kBlock / tpr, want = (rows + teams - 1) / teams;
+  return (uint32_t)(want < 8192 ? want : 8192);
+}
+
+}  // namespace
+
+hipError_t act8_pack(const Act8Move& a, hipStream_t stream) {
+  if (a.rows == 0 || a.cols == 0) return hipSuccess;
+  const int tpr = team_size(a.pitch);
+  with_type(a.type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    launch(act8_pack_kernel<T>, row_grid(a.rows, tpr), kBlock, stream, a, tpr);
+  });
+  return hipGetLastError();
+}
+
+hipError_t act8_unpack(const Act8Move& a, hipStream_t stream) {
+  if (a.rows == 0 || a.cols == 0) return hipSuccess;
+  const int tpr = team_size(a.pitch);
+  with_type(a.type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    launch(act8_unpack_kernel<T>, row_grid(a.rows, tpr), kBlock, stream, a, tpr);
+  });
+  return hipGetLastError();
+}
+
+hipError_t silu_act8_forward(const SiluAct8& p, hipStream_t stream) {
+  if (p.rows == 0 || p.cols == 0) return hipSuccess;
+  const int tpr = team_size(p.pitch);
+  with_type(p.type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    launch(silu_forward_kernel<T>, row_grid(p.rows, tpr), kBlock, stream, p, tpr);
+  });
+  return hipGetLastError();
+}
+
+hipError_t silu_act8_backward(const SiluAct8& p, hipStream_t stream) {
+  if (p.rows == 0 || p.cols == 0) return hipSuccess;
+  const int tpr = team_size(p.pitch);
+  with_type(p.type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    launch(silu_backward_kernel<T>, row_grid(p.rows, tpr), kBlock, stream, p, tpr);
+  });
+  return hipGetLastError();
+}
+
+}  // namespace baguanet

@@ -188,7 +188,12 @@ void fused_sgd(std::vector<torch::Tensor> params,
 }  // namespace
 }  // namespace baguanet
 
+namespace baguanet {
+void bind_train_ops(pybind11::module& m);  // train_ops.cc
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  baguanet::bind_train_ops(m);
   m.def("copy_bytes", &baguanet::copy_bytes,
         "vectorized gfx950 copy kernel (dst, src)");
   m.def("multi_pack", &baguanet::multi_pack,

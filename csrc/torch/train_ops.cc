@@ -1,0 +1,752 @@
+// train_ops.cc — torch bindings and autograd of the training-step kernels:
+// embedding, gated residual norm, 8-bit activation checkpoints.
+//
+// Arguments are checked in the order type, shape, size, device, so that a
+// wrong call is refused the same way with or without a GPU.  Kernels run on
+// the current stream of their tensors' device; workspaces and saved tensors
+// come from torch's allocator, so calls may be captured into a graph.
+
+#include <c10/core/DeviceGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/extension.h>
+
+#include <optional>
+#include <tuple>
+#include <vector>
+
+#include "../hip/train_kernels.h"
+
+namespace baguanet {
+namespace {
+
+using torch::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<Tensor>;
+
+constexpr int64_t kMaxRows = int64_t(1) << 30;
+
+hipStream_t stream_of(const Tensor& t) {
+  return (hipStream_t)c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
+}
+
+void check_launch(hipError_t e, const char* what) {
+  TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e));
+}
+
+bool is_act_type(at::ScalarType t) {
+  return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf;
+}
+
+ElemType elem(at::ScalarType t) {
+  return t == at::kFloat      ? ElemType::kF32
+         : t == at::kBFloat16 ? ElemType::kBF16
+                              : ElemType::kF16;
+}
+
+void check_act(const Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(t.defined(), op, ": ", name, " is missing");
+  TORCH_CHECK(t.layout() == at::kStrided, op, ": ", name, " must be dense");
+  TORCH_CHECK(is_act_type(t.scalar_type()), op, ": ", name,
+              " must be float32, bfloat16 or float16, not ", t.scalar_type());
+}
+
+void check_device(const Tensor& t, const Tensor& on, const char* op,
+                  const char* name) {
+  TORCH_CHECK(t.is_cuda(), op, ": ", name, " must be on the GPU");
+  TORCH_CHECK(t.device() == on.device(), op, ": ", name, " is on ",
+              t.device(), ", expected ", on.device());
+}
+
+void no_double_backward(const char* op) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), op,
+              ": its gradient cannot be differentiated again");
+}
+
+// A tensor as rows of its last dimension: unit stride within a row and one
+// stride between rows.  Others are copied.
+struct Rows {
+  Tensor t;
+  int64_t stride;
+};
+
+Rows as_rows(const Tensor& t) {
+  const int64_t dim = t.size(-1);
+  bool ok = dim <= 1 || t.stride(-1) == 1;
+  int64_t stride = dim, next = -1;
+  for (int64_t d = t.dim() - 2; d >= 0 && ok; d--) {
+    if (t.size(d) == 1) continue;
+    if (next < 0)
+      stride = t.stride(d);
+    else
+      ok = t.stride(d) == next;
+    next = t.stride(d) * t.size(d);
+  }
+  if (ok) return {t, stride};
+  return {t.contiguous(), dim};
+}
+
+int64_t rows_of(const Tensor& t) {
+  int64_t r = 1;
+  for (int64_t d = 0; d < t.dim() - 1; d++) r *= t.size(d);
+  return r;
+}
+
+Tensor empty_bytes(size_t bytes, const Tensor& like) {
+  return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+}
+
+Tensor or_undefined(const OptTensor& t) { return t ? *t : Tensor(); }
+
+// ---------------------------------------------------------------------------
+// embedding
+
+struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight,
+                        const Tensor& tokens, double scale, int64_t padding,
+                        int64_t out_type) {
+    const c10::OptionalDeviceGuard guard(weight.device());
+    const Tensor w = weight.stride(-1) == 1 ? weight : weight.contiguous();
+    const Tensor tok = tokens.contiguous();
+    auto sizes = tokens.sizes().vec();
+    sizes.push_back(weight.size(1));
+    Tensor out = at::empty(
+        sizes, weight.options().dtype((at::ScalarType)out_type));
+    EmbeddingFwd a = {};
+    a.weight = w.data_ptr();
+    a.tokens = tok.data_ptr();
+    a.out = out.data_ptr();
+    a.vocab = w.size(0);
+    a.dim = w.size(1);
+    a.n = tok.numel();
+    a.wstride = w.stride(0);
+    a.scale = (float)scale;
+    a.tok64 = tok.scalar_type() == at::kLong;
+    a.wtype = elem(w.scalar_type());
+    a.otype = elem(out.scalar_type());
+    check_launch(embedding_forward(a, stream_of(w)), "embedding");
+    ctx->save_for_backward({tok});
+    ctx->saved_data["vocab"] = w.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    ctx->saved_data["type"] = (int64_t)w.scalar_type();
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_double_backward("embedding");
+    const Tensor tok = ctx->get_saved_variables()[0];
+    const Rows dout = as_rows(grads[0]);
+    const c10::OptionalDeviceGuard guard(dout.t.device());
+    EmbeddingBwd a = {};
+    a.vocab = ctx->saved_data["vocab"].toInt();
+    a.dim = dout.t.size(-1);
+    a.n = tok.numel();
+    Tensor dw = at::empty(
+        {a.vocab, a.dim},
+        dout.t.options().dtype(
+            (at::ScalarType)ctx->saved_data["type"].toInt()));
+    const Tensor ws =
+        empty_bytes(embedding_workspace(a.vocab, a.dim, a.n), dout.t);
+    a.dout = dout.t.data_ptr();
+    a.tokens = tok.data_ptr();
+    a.dweight = dw.data_ptr();
+    a.workspace = ws.data_ptr();
+    a.dstride = dout.stride;
+    a.padding = ctx->saved_data["padding"].toInt();
+    a.scale = (float)ctx->saved_data["scale"].toDouble();
+    a.tok64 = tok.scalar_type() == at::kLong;
+    a.dtype = elem(dout.t.scalar_type());
+    a.wtype = elem(dw.scalar_type());
+    check_launch(embedding_backward(a, stream_of(dw)), "embedding backward");
+    return {dw, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor embedding(const Tensor& weight, const Tensor& tokens, double scale,
+                 std::optional<int64_t> padding_idx,
+                 std::optional<at::ScalarType> out_dtype) {
+  const char* op = "embedding";
+  check_act(weight, op, "weight");
+  TORCH_CHECK(tokens.scalar_type() == at::kLong ||
+                  tokens.scalar_type() == at::kInt,
+              op, ": tokens must be int64 or int32, not ",
+              tokens.scalar_type());
+  const at::ScalarType out = out_dtype ? *out_dtype : weight.scalar_type();
+  TORCH_CHECK(is_act_type(out), op,
+              ": out_dtype must be float32, bfloat16 or float16, not ", out);
+  TORCH_CHECK(weight.dim() == 2, op, ": weight must be [vocab, dim], not ",
+              weight.sizes());
+  const int64_t vocab = weight.size(0);
+  TORCH_CHECK(vocab <= kMaxRows && tokens.numel() <= kMaxRows, op,
+              ": at most 2^30 rows and tokens");
+  int64_t padding = -1;
+  if (padding_idx) {
+    padding = *padding_idx < 0 ? *padding_idx + vocab : *padding_idx;
+    TORCH_CHECK(padding >= 0 && padding < vocab, op, ": padding_idx ",
+                *padding_idx, " is outside a table of ", vocab, " rows");
+  }
+  check_device(weight, weight, op, "weight");
+  check_device(tokens, weight, op, "tokens");
+  return EmbeddingFn::apply(weight, tokens, scale, padding, (int64_t)out);
+}
+
+// ---------------------------------------------------------------------------
+// gated residual norm
+
+struct NormFn : torch::autograd::Function<NormFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x,
+                               const OptTensor& branch_, const OptTensor& gate_,
+                               const OptTensor& post_, const OptTensor& pre_,
+                               double residual_scale, double branch_scale,
+                               double eps, int64_t gmode, int64_t group_rows,
+                               bool want_h) {
+    const c10::OptionalDeviceGuard guard(x.device());
+    const Tensor branch = or_undefined(branch_), pre = or_undefined(pre_);
+    const Tensor gate = or_undefined(gate_), post = or_undefined(post_);
+    const Rows xr = as_rows(x);
+    NormFwd a = {};
+    a.rows = rows_of(x);
+    a.dim = x.size(-1);
+    a.x = xr.t.data_ptr();
+    a.xstride = xr.stride;
+    a.type = elem(x.scalar_type());
+    a.residual_scale = (float)residual_scale;
+    a.branch_scale = (float)branch_scale;
+    a.eps = (float)eps;
+    a.gmode = (Gate)gmode;
+    a.group_rows = group_rows;
+    const auto stats = x.options().dtype(at::kFloat);
+    Tensor y, h, rbranch, ry;
+    Rows br;
+    if (branch.defined()) {
+      br = as_rows(branch);
+      a.branch = br.t.data_ptr();
+      a.bstride = br.stride;
+      y = at::empty(x.sizes(), x.options());
+      a.y = y.data_ptr();
+      if (gate.defined()) {
+        a.gate = gate.data_ptr();
+        a.gate32 = gate.scalar_type() == at::kFloat;
+      }
+      if (post.defined()) {
+        a.post = post.data_ptr();
+        a.post32 = post.scalar_type() == at::kFloat;
+        rbranch = at::empty({a.rows}, stats);
+        a.rbranch = rbranch.data_ptr<float>();
+      }
+    }
+    if (want_h) {
+      h = at::empty(x.sizes(), x.options());
+      a.h = h.data_ptr();
+      ry = at::empty({a.rows}, stats);
+      a.ry = ry.data_ptr<float>();
+      if (pre.defined()) {
+        a.pre = pre.data_ptr();
+        a.pre32 = pre.scalar_type() == at::kFloat;
+      }
+    }
+    check_launch(norm_forward(a, stream_of(x)), "residual norm");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({branch.defined() ? y : want_h ? xr.t : Tensor(),
+                            branch.defined() ? br.t : Tensor(), gate, post,
+                            pre, rbranch, ry});
+    ctx->saved_data["scales"] =
+        std::vector<double>{residual_scale, branch_scale};
+    ctx->saved_data["gate"] = std::vector<int64_t>{gmode, group_rows};
+    ctx->saved_data["needs"] = std::vector<int64_t>{
+        gate.defined() && gate.requires_grad(),
+        post.defined() && post.requires_grad(),
+        pre.defined() && pre.requires_grad()};
+    variable_list out;
+    if (y.defined()) out.push_back(y);
+    if (h.defined()) out.push_back(h);
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_double_backward("residual norm");
+    variable_list out(11);
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &y = saved[0], &branch = saved[1], &gate = saved[2],
+                 &post = saved[3], &pre = saved[4], &rbranch = saved[5],
+                 &ry = saved[6];
+    Tensor dy, dh;
+    if (branch.defined()) {
+      dy = grads[0];
+      if (grads.size() > 1) dh = grads[1];
+    } else {
+      dh = grads[0];
+    }
+    if (!dy.defined() && !dh.defined()) return out;
+    const Tensor& some = dy.defined() ? dy : dh;
+    const c10::OptionalDeviceGuard guard(some.device());
+    NormBwd a = {};
+    a.rows = rows_of(some);
+    a.dim = some.size(-1);
+    a.type = elem(some.scalar_type());
+    const auto scales = ctx->saved_data["scales"].toDoubleVector();
+    const auto g = ctx->saved_data["gate"].toIntVector();
+    const auto needs = ctx->saved_data["needs"].toIntVector();
+    a.residual_scale = (float)scales[0];
+    a.branch_scale = (float)scales[1];
+    a.gmode = (Gate)g[0];
+    a.group_rows = g[1];
+    Rows yr, br, dyr, dhr;
+    Tensor dx = at::empty(some.sizes(), some.options());
+    a.dx = dx.data_ptr();
+    Tensor dbranch, dgate, dpost, dpre;
+    if (dy.defined()) {
+      dyr = as_rows(dy);
+      a.dy = dyr.t.data_ptr();
+      a.dystride = dyr.stride;
+    }
+    if (dh.defined()) {
+      yr = as_rows(y);
+      dhr = as_rows(dh);
+      a.y = yr.t.data_ptr();
+      a.ystride = yr.stride;
+      a.dh = dhr.t.data_ptr();
+      a.dhstride = dhr.stride;
+      a.ry = ry.data_ptr<float>();
+      if (pre.defined()) {
+        a.pre = pre.data_ptr();
+        a.pre32 = pre.scalar_type() == at::kFloat;
+        if (needs[2]) {
+          dpre = at::empty(pre.sizes(), pre.options());
+          a.dpre = dpre.data_ptr();
+        }
+      }
+    }
+    if (branch.defined()) {
+      br = as_rows(branch);
+      a.branch = br.t.data_ptr();
+      a.bstride = br.stride;
+      dbranch = at::empty(some.sizes(), some.options());
+      a.dbranch = dbranch.data_ptr();
+      if (gate.defined()) {
+        a.gate = gate.data_ptr();
+        a.gate32 = gate.scalar_type() == at::kFloat;
+        if (needs[0]) {
+          dgate = at::empty(gate.sizes(), gate.options());
+          a.dgate = dgate.data_ptr();
+        }
+      }
+      if (post.defined()) {
+        a.post = post.data_ptr();
+        a.post32 = post.scalar_type() == at::kFloat;
+        a.rbranch = rbranch.data_ptr<float>();
+        if (needs[1]) {
+          dpost = at::empty(post.sizes(), post.options());
+          a.dpost = dpost.data_ptr();
+        }
+      }
+    }
+    if (a.rows == 0 || a.dim == 0) {
+      for (Tensor* t : {&dgate, &dpost, &dpre})
+        if (t->defined()) t->zero_();
+    }
+    const Tensor ws = empty_bytes(norm_workspace(a), dx);
+    a.workspace = ws.data_ptr();
+    check_launch(norm_backward(a, stream_of(dx)), "residual norm backward");
+    out[0] = dx;
+    out[1] = dbranch;
+    out[2] = dgate;
+    out[3] = dpost;
+    out[4] = dpre;
+    return out;
+  }
+};
+
+void check_norm_input(const Tensor& x, const char* op, const char* name) {
+  check_act(x, op, name);
+  TORCH_CHECK(x.dim() >= 1, op, ": ", name, " must have rows, not be a scalar");
+  TORCH_CHECK(x.size(-1) <= kNormMaxDim, op, ": rows of at most ", kNormMaxDim,
+              " columns, not ", x.size(-1));
+  TORCH_CHECK(rows_of(x) <= kMaxRows, op, ": at most 2^30 rows");
+}
+
+void check_norm_weight(const OptTensor& w, const Tensor& x, const char* op,
+                       const char* name) {
+  if (!w) return;
+  check_act(*w, op, name);
+  TORCH_CHECK(w->scalar_type() == at::kFloat ||
+                  w->scalar_type() == x.scalar_type(),
+              op, ": ", name, " must be float32 or of x's type, not ",
+              w->scalar_type());
+  TORCH_CHECK(w->dim() == 1 && w->size(0) == x.size(-1), op, ": ", name,
+              " must be [", x.size(-1), "], not ", w->sizes());
+}
+
+OptTensor contiguous(const OptTensor& t) {
+  return t ? OptTensor(t->contiguous()) : OptTensor();
+}
+
+Tensor rms_norm(const Tensor& x, const OptTensor& weight, double eps) {
+  const char* op = "rms_norm";
+  check_norm_input(x, op, "x");
+  check_norm_weight(weight, x, op, "weight");
+  TORCH_CHECK(eps >= 0, op, ": eps must not be negative");
+  check_device(x, x, op, "x");
+  if (weight) check_device(*weight, x, op, "weight");
+  return NormFn::apply(x, OptTensor(), OptTensor(), OptTensor(),
+                       contiguous(weight), 1.0, 1.0, eps, (int64_t)Gate::kNone,
+                       int64_t(1), true)[0];
+}
+
+std::tuple<Tensor, OptTensor> gated_residual_norm(
+    const Tensor& x, const Tensor& branch, const OptTensor& gate,
+    const OptTensor& post_weight, const OptTensor& pre_weight,
+    double residual_scale, double branch_scale, double eps) {
+  const char* op = "gated_residual_norm";
+  check_norm_input(x, op, "x");
+  check_act(branch, op, "branch");
+  TORCH_CHECK(branch.scalar_type() == x.scalar_type(), op,
+              ": branch must have x's type ", x.scalar_type(), ", not ",
+              branch.scalar_type());
+  TORCH_CHECK(branch.sizes() == x.sizes(), op, ": branch must have x's shape ",
+              x.sizes(), ", not ", branch.sizes());
+  check_norm_weight(post_weight, x, op, "post_weight");
+  check_norm_weight(pre_weight, x, op, "pre_weight");
+  TORCH_CHECK(eps >= 0, op, ": eps must not be negative");
+  const int64_t dim = x.size(-1), rows = rows_of(x);
+  Gate mode = Gate::kNone;
+  int64_t group_rows = rows > 0 ? rows : 1;
+  OptTensor g;
+  if (gate) {
+    check_act(*gate, op, "gate");
+    TORCH_CHECK(gate->scalar_type() == at::kFloat ||
+                    gate->scalar_type() == x.scalar_type(),
+                op, ": gate must be float32 or of x's type, not ",
+                gate->scalar_type());
+    bool fits = gate->dim() <= x.dim();
+    for (int64_t d = 1; fits && d <= gate->dim(); d++)
+      fits = gate->size(-d) == 1 || gate->size(-d) == x.size(-d);
+    TORCH_CHECK(fits, op, ": gate ", gate->sizes(),
+                " cannot be broadcast to x ", x.sizes());
+    // x's leading dimensions that the gate has too, then those it lacks
+    std::vector<int64_t> lead(x.dim() - 1, 1);
+    for (int64_t d = 0; d < gate->dim() - 1; d++)
+      lead[lead.size() - 1 - d] = gate->size(gate->dim() - 2 - d);
+    const bool wide = gate->dim() > 0 && gate->size(-1) == dim;
+    size_t own = 0;
+    while (own < lead.size() && lead[own] == x.size(own)) own++;
+    bool prefix = true;
+    for (size_t d = own; d < lead.size(); d++) prefix &= lead[d] == 1;
+    Tensor t = *gate;
+    if (wide && prefix) {
+      group_rows = 1;
+      for (size_t d = own; d < lead.size(); d++) group_rows *= x.size(d);
+      mode = group_rows == 1 && rows > 1 ? Gate::kFull : Gate::kGroup;
+      if (group_rows == 0) group_rows = 1;
+    } else {
+      // one value for each row, or any other pattern element by element;
+      // autograd sums the gradient back over what is repeated here
+      auto to = x.sizes().vec();
+      mode = wide ? Gate::kFull : Gate::kRow;
+      if (!wide) to.back() = 1;
+      t = t.expand(to);
+    }
+    g = t.contiguous();
+  }
+  check_device(x, x, op, "x");
+  check_device(branch, x, op, "branch");
+  if (gate) check_device(*gate, x, op, "gate");
+  if (post_weight) check_device(*post_weight, x, op, "post_weight");
+  if (pre_weight) check_device(*pre_weight, x, op, "pre_weight");
+  auto out = NormFn::apply(x, branch, g, contiguous(post_weight),
+                           contiguous(pre_weight), residual_scale,
+                           branch_scale, eps, (int64_t)mode, group_rows,
+                           pre_weight.has_value());
+  return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
+}
+
+// ---------------------------------------------------------------------------
+// 8-bit activation checkpoints
+
+int64_t pitch_of(int64_t cols) {
+  return (cols + kAct8Group - 1) / kAct8Group * kAct8Group;
+}
+
+void check_act8_input(const Tensor& x, const char* op, const char* name) {
+  check_act(x, op, name);
+  TORCH_CHECK(x.dim() >= 1, op, ": ", name, " must have rows, not be a scalar");
+  TORCH_CHECK(rows_of(x) <= kMaxRows && x.size(-1) <= kMaxRows, op,
+              ": at most 2^30 rows and columns");
+}
+
+std::tuple<Tensor, Tensor> pack_rows(const Tensor& x) {
+  const c10::OptionalDeviceGuard guard(x.device());
+  const Rows xr = as_rows(x);
+  Act8Move a = {};
+  a.rows = rows_of(x);
+  a.cols = x.size(-1);
+  a.pitch = pitch_of(a.cols);
+  const auto bytes = x.options().dtype(at::kByte);
+  Tensor codes = at::empty({a.rows, a.pitch}, bytes);
+  Tensor exps = at::empty({a.rows, a.pitch / kAct8Group}, bytes);
+  a.x = xr.t.data_ptr();
+  a.xstride = xr.stride;
+  a.codes = codes.data_ptr<uint8_t>();
+  a.exps = exps.data_ptr<uint8_t>();
+  a.type = elem(x.scalar_type());
+  check_launch(act8_pack(a, stream_of(x)), "act8_pack");
+  return {codes, exps};
+}
+
+std::tuple<Tensor, Tensor> act8_pack_op(const Tensor& x) {
+  check_act8_input(x, "act8_pack", "x");
+  check_device(x, x, "act8_pack", "x");
+  at::NoGradGuard no_grad;
+  return pack_rows(x.detach());
+}
+
+// A checkpoint's parts against the rows and columns they stand for.
+void check_codes(const Tensor& codes, const Tensor& exps, int64_t rows,
+                 int64_t cols, const char* op) {
+  const int64_t pitch = pitch_of(cols);
+  TORCH_CHECK(codes.scalar_type() == at::kByte &&
+                  exps.scalar_type() == at::kByte,
+              op, ": codes and exponents must be bytes");
+  TORCH_CHECK(codes.dim() == 2 && codes.size(0) == rows &&
+                  codes.size(1) == pitch && codes.is_contiguous(),
+              op, ": codes must be contiguous [", rows, ", ", pitch, "], not ",
+              codes.sizes());
+  TORCH_CHECK(exps.dim() == 2 && exps.size(0) == rows &&
+                  exps.size(1) == pitch / kAct8Group && exps.is_contiguous(),
+              op, ": exponents must be contiguous [", rows, ", ",
+              pitch / kAct8Group, "], not ", exps.sizes());
+}
+
+void check_codes_aligned(const Tensor& codes, const char* op) {
+  TORCH_CHECK(((uintptr_t)codes.data_ptr() & 15) == 0, op,
+              ": codes must be aligned to 16 bytes");
+}
+
+Tensor act8_unpack_op(const Tensor& codes, const Tensor& exps,
+                      const std::vector<int64_t>& shape,
+                      at::ScalarType dtype) {
+  const char* op = "act8_unpack";
+  TORCH_CHECK(is_act_type(dtype), op,
+              ": dtype must be float32, bfloat16 or float16, not ", dtype);
+  TORCH_CHECK(!shape.empty(), op, ": the shape must have rows");
+  int64_t rows = 1;
+  for (size_t d = 0; d + 1 < shape.size(); d++) rows *= shape[d];
+  check_codes(codes, exps, rows, shape.back(), op);
+  check_device(codes, codes, op, "codes");
+  check_device(exps, codes, op, "exponents");
+  check_codes_aligned(codes, op);
+  const c10::OptionalDeviceGuard guard(codes.device());
+  Tensor x = at::empty(shape, codes.options().dtype(dtype));
+  Act8Move a = {};
+  a.x = x.data_ptr();
+  a.codes = codes.data_ptr<uint8_t>();
+  a.exps = exps.data_ptr<uint8_t>();
+  a.rows = rows;
+  a.cols = a.xstride = shape.back();
+  a.pitch = pitch_of(a.cols);
+  a.type = elem(dtype);
+  check_launch(act8_unpack(a, stream_of(x)), op);
+  return x;
+}
+
+std::tuple<Tensor, Tensor> wgrad_rows(const Tensor& dy, const Tensor& codes,
+                                      const Tensor& exps, int64_t k,
+                                      bool bias) {
+  const c10::OptionalDeviceGuard guard(dy.device());
+  const Rows dr = as_rows(dy);
+  Act8Wgrad a = {};
+  a.m = rows_of(dy);
+  a.n = dy.size(-1);
+  a.k = k;
+  a.pitch = pitch_of(k);
+  Tensor dw = at::empty({a.n, a.k}, dy.options());
+  Tensor db = bias ? at::empty({a.n}, dy.options()) : Tensor();
+  if (a.m == 0) dw.zero_();
+  if (bias && (a.m == 0 || a.k == 0)) db.copy_(dy.reshape({-1, a.n}).sum(0));
+  a.dy = dr.t.data_ptr();
+  a.dstride = dr.stride;
+  a.codes = codes.data_ptr<uint8_t>();
+  a.exps = exps.data_ptr<uint8_t>();
+  a.dw = dw.data_ptr();
+  a.db = bias ? db.data_ptr() : nullptr;
+  a.type = elem(dy.scalar_type());
+  const Tensor ws = empty_bytes(act8_wgrad_workspace(a), dy);
+  a.workspace = ws.data_ptr();
+  check_launch(act8_wgrad(a, stream_of(dy)), "act8_wgrad");
+  return {dw, db};
+}
+
+std::tuple<Tensor, OptTensor> act8_wgrad_op(const Tensor& dy,
+                                            const Tensor& codes,
+                                            const Tensor& exps,
+                                            const std::vector<int64_t>& shape,
+                                            at::ScalarType dtype, bool bias) {
+  const char* op = "act8_wgrad";
+  check_act8_input(dy, op, "dy");
+  TORCH_CHECK(dy.scalar_type() == dtype, op, ": dy must have the kept input's "
+              "type ", dtype, ", not ", dy.scalar_type());
+  TORCH_CHECK((size_t)dy.dim() == shape.size(), op, ": dy ", dy.sizes(),
+              " does not have the rows of the kept input ",
+              at::IntArrayRef(shape));
+  for (size_t d = 0; d + 1 < shape.size(); d++)
+    TORCH_CHECK(dy.size(d) == shape[d], op, ": dy ", dy.sizes(),
+                " does not have the rows of the kept input ",
+                at::IntArrayRef(shape));
+  check_codes(codes, exps, rows_of(dy), shape.back(), op);
+  check_device(dy, dy, op, "dy");
+  check_device(codes, dy, op, "codes");
+  check_device(exps, dy, op, "exponents");
+  check_codes_aligned(codes, op);
+  at::NoGradGuard no_grad;
+  auto [dw, db] = wgrad_rows(dy.detach(), codes, exps, shape.back(), bias);
+  return {dw, bias ? OptTensor(db) : OptTensor()};
+}
+
+// A linear layer whose input is kept in 8 bits.  Its two plain products, y
+// and dx, are the library's, as in torch.nn.Linear; the weight gradient is
+// taken from the codes.
+struct LinearAct8Fn : torch::autograd::Function<LinearAct8Fn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x,
+                        const Tensor& weight, const OptTensor& bias) {
+    const c10::OptionalDeviceGuard guard(x.device());
+    Tensor codes, exps;
+    const bool grad_b = bias && bias->requires_grad();
+    if (weight.requires_grad()) std::tie(codes, exps) = pack_rows(x);
+    ctx->save_for_backward(
+        {x.requires_grad() ? weight : Tensor(), codes, exps});
+    ctx->saved_data["needs"] = std::vector<int64_t>{
+        x.requires_grad(), weight.requires_grad(), grad_b};
+    ctx->saved_data["k"] = x.size(-1);
+    return at::linear(x, weight, bias);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_double_backward("linear_act8");
+    const auto saved = ctx->get_saved_variables();
+    const auto needs = ctx->saved_data["needs"].toIntVector();
+    const Tensor& dy = grads[0];
+    const c10::OptionalDeviceGuard guard(dy.device());
+    variable_list out(3);
+    if (needs[0]) out[0] = at::matmul(dy, saved[0]);
+    if (needs[1])
+      std::tie(out[1], out[2]) =
+          wgrad_rows(dy, saved[1], saved[2], ctx->saved_data["k"].toInt(),
+                     needs[2]);
+    else if (needs[2])
+      out[2] = dy.reshape({-1, dy.size(-1)}).sum(0);
+    return out;
+  }
+};
+
+Tensor linear_act8(const Tensor& x, const Tensor& weight,
+                   const OptTensor& bias) {
+  const char* op = "linear_act8";
+  check_act8_input(x, op, "x");
+  check_act(weight, op, "weight");
+  TORCH_CHECK(weight.scalar_type() == x.scalar_type(), op,
+              ": weight must have x's type ", x.scalar_type(), ", not ",
+              weight.scalar_type());
+  TORCH_CHECK(weight.dim() == 2 && weight.size(1) == x.size(-1), op,
+              ": weight must be [out, ", x.size(-1), "], not ",
+              weight.sizes());
+  if (bias) {
+    check_act(*bias, op, "bias");
+    TORCH_CHECK(bias->scalar_type() == x.scalar_type(), op,
+                ": bias must have x's type ", x.scalar_type(), ", not ",
+                bias->scalar_type());
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == weight.size(0), op,
+                ": bias must be [", weight.size(0), "], not ", bias->sizes());
+  }
+  check_device(x, x, op, "x");
+  check_device(weight, x, op, "weight");
+  if (bias) check_device(*bias, x, op, "bias");
+  return LinearAct8Fn::apply(x, weight, bias);
+}
+
+struct SiluAct8Fn : torch::autograd::Function<SiluAct8Fn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x) {
+    const c10::OptionalDeviceGuard guard(x.device());
+    const Rows xr = as_rows(x);
+    SiluAct8 p = {};
+    p.rows = rows_of(x);
+    p.cols = x.size(-1) / 2;
+    p.pitch = pitch_of(p.cols);
+    p.x = xr.t.data_ptr();
+    p.xstride = xr.stride;
+    p.type = elem(x.scalar_type());
+    auto sizes = x.sizes().vec();
+    sizes.back() = p.cols;
+    Tensor out = at::empty(sizes, x.options()), codes, exps;
+    p.out = out.data_ptr();
+    if (x.requires_grad()) {
+      const auto bytes = x.options().dtype(at::kByte);
+      codes = at::empty({p.rows, 2 * p.pitch}, bytes);
+      exps = at::empty({p.rows, 2 * p.pitch / kAct8Group}, bytes);
+      p.codes = codes.data_ptr<uint8_t>();
+      p.exps = exps.data_ptr<uint8_t>();
+    }
+    check_launch(silu_act8_forward(p, stream_of(x)), "silu_mul_act8");
+    ctx->save_for_backward({codes, exps});
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_double_backward("silu_mul_act8");
+    const auto saved = ctx->get_saved_variables();
+    const Rows dr = as_rows(grads[0]);
+    const c10::OptionalDeviceGuard guard(dr.t.device());
+    SiluAct8 p = {};
+    p.rows = rows_of(dr.t);
+    p.cols = dr.t.size(-1);
+    p.pitch = pitch_of(p.cols);
+    p.dout = dr.t.data_ptr();
+    p.dstride = dr.stride;
+    p.type = elem(dr.t.scalar_type());
+    auto sizes = dr.t.sizes().vec();
+    sizes.back() = 2 * p.cols;
+    Tensor dx = at::empty(sizes, dr.t.options());
+    p.dx = dx.data_ptr();
+    p.codes = saved[0].data_ptr<uint8_t>();
+    p.exps = saved[1].data_ptr<uint8_t>();
+    check_launch(silu_act8_backward(p, stream_of(dx)),
+                 "silu_mul_act8 backward");
+    return {dx};
+  }
+};
+
+Tensor silu_mul_act8(const Tensor& x) {
+  const char* op = "silu_mul_act8";
+  check_act8_input(x, op, "x");
+  TORCH_CHECK(x.size(-1) % 2 == 0, op,
+              ": x must hold two halves in its last dimension, not ",
+              x.size(-1), " columns");
+  check_device(x, x, op, "x");
+  return SiluAct8Fn::apply(x);
+}
+
+}  // namespace
+
+void bind_train_ops(pybind11::module& m) {
+  namespace py = pybind11;
+  m.def("embedding", &embedding, "scaled lookup of table rows",
+        py::arg("weight"), py::arg("tokens"), py::arg("scale"),
+        py::arg("padding_idx"), py::arg("out_dtype"));
+  m.def("rms_norm", &rms_norm, "norm before a block", py::arg("x"),
+        py::arg("weight"), py::arg("eps"));
+  m.def("gated_residual_norm", &gated_residual_norm,
+        "norm after a block, gate, residual scale and the next block's norm",
+        py::arg("x"), py::arg("branch"), py::arg("gate"),
+        py::arg("post_weight"), py::arg("pre_weight"),
+        py::arg("residual_scale"), py::arg("branch_scale"), py::arg("eps"));
+  m.def("act8_pack", &act8_pack_op, "8-bit copy of an activation");
+  m.def("act8_unpack", &act8_unpack_op, "the values an 8-bit copy stands for");
+  m.def("act8_wgrad", &act8_wgrad_op,
+        "a linear layer's weight gradient from its input's 8-bit copy");
+  m.def("linear_act8", &linear_act8, "linear layer, its input kept in 8 bits",
+        py::arg("x"), py::arg("weight"), py::arg("bias"));
+  m.def("silu_mul_act8", &silu_mul_act8,
+        "silu(a) * b, its inputs kept in 8 bits");
+}
+
+}  // namespace baguanet

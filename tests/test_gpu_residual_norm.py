@@ -1,0 +1,370 @@
+"""baguanet.ops.rms_norm and gated_residual_norm against their definition in
+64 bits.
+
+Tolerances: outputs are rounded once to their type (half a step: eps / 2 of
+the value, and half of float16's smallest step of 2**-24).  Before that all is
+fp32: a sum of at most 32768 terms goes through fewer than 48 additions on any
+path (8 of a vector, 4 vectors, 6 lane exchanges, 16 waves), and the products
+around it add fewer than 16 roundings, so C = 64 half steps of 2**-24, relative
+to the sum of the magnitudes, bound each number before its last rounding.  The
+backward pass reads y as it was rounded, so what it takes from y carries half
+a step of the type more.  Sums over R rows add R roundings.
+"""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+U = 2.0 ** -24
+C = 64 * U
+
+
+def check(got, ref, extra, what):
+    d = got.dtype
+    assert got.shape == ref.shape, what
+    got = got.detach().double().cpu()
+    tol = (ref.abs() * torch.finfo(d).eps / 2 * (1 + C) + extra * (1 + 2 ** -6)
+           + 2.0 ** -25 * (d == HF) + 1e-37)
+    off = (got - ref).abs()
+    assert (off <= tol).all(), (what, (off / tol).max().item())
+
+
+def reference(x, o, gate, post, pre, rs, bs, eps, dy, dh, half):
+    """Values, gradients and how far each may be off before its rounding.
+
+    `half`: half a step of the activations' type, relative.
+    """
+    dim = x.shape[-1]
+    x, o = x.double(), o.double()
+    one = torch.ones((), dtype=torch.float64)
+    g = one if gate is None else gate.double()
+    wp = one if post is None else post.double()
+    wn = one if pre is None else pre.double()
+    ro = one
+    if post is not None:
+        ro = (o.pow(2).mean(-1, keepdim=True) + eps).rsqrt()
+    no = o * ro
+    u = no * wp
+    y = rs * x + bs * g * u
+    e_y = C * ((rs * x).abs() + (bs * g * u).abs())
+    out = {"y": (y, e_y)}
+    ry = (y.pow(2).mean(-1, keepdim=True) + eps).rsqrt()
+    ny = y * ry
+    if pre is not None:
+        rel = (y.abs() * e_y).mean(-1, keepdim=True) * ry ** 2 + C
+        h = ny * wn
+        out["h"] = (h, (wn * ry).abs() * e_y + h.abs() * rel)
+    dy = torch.zeros_like(x) if dy is None else dy.double()
+    t = torch.zeros_like(x)
+    if pre is not None and dh is not None:
+        dh = dh.double()
+        t = dh * wn
+    # relative errors of ny as the backward pass has it
+    rel = (y.abs() * e_y).mean(-1, keepdim=True) * ry ** 2
+    r_ny = half + C + rel
+    mean = (ny * t).mean(-1, keepdim=True)
+    mean_abs = (ny * t).abs().mean(-1, keepdim=True)
+    d = dy + ry * (t - ny * mean)
+    d_abs = dy.abs() + ry * (t.abs() + ny.abs() * mean_abs)
+    e_d = (C + rel) * d_abs + 2 * ry * ny.abs() * mean_abs * r_ny
+    out["dx"] = (rs * d, abs(rs) * e_d)
+    c = bs * g * wp
+    if post is None:
+        out["dbranch"] = (c * d, c.abs() * (e_d + C * d_abs))
+    else:
+        mean = (no * c * d).mean(-1, keepdim=True)
+        e_in = (e_d + C * d_abs) * c.abs()
+        e_mean = (no.abs() * e_in).mean(-1, keepdim=True)
+        # the kernel's mean is a difference of two sums of these magnitudes
+        e_mean = e_mean + (ny * no * c).abs().mean(-1, keepdim=True) * (
+            ry * mean_abs * (C + 2 * r_ny))
+        out["dbranch"] = (ro * (c * d - no * mean),
+                          ro * (e_in + no.abs() * (e_mean + C * mean.abs())))
+    rows = x.numel() // dim
+    flat = lambda v: v.expand_as(x).reshape(-1, dim)
+    if pre is not None and dh is not None:
+        p = dh * ny
+        out["dpre"] = (flat(p).sum(0),
+                       flat(p.abs() * (r_ny + C + rows * U)).sum(0))
+    if post is not None:
+        p = bs * g * d * no
+        e = (bs * g * no).abs() * (e_d + (C + rows * U) * d_abs)
+        out["dpost"] = (flat(p).sum(0), flat(e).sum(0))
+    if gate is not None:
+        p = bs * d * u
+        e = (bs * u).abs() * (e_d + (C + (rows + dim) * U) * d_abs)
+        if gate.shape[-1:] == (1,) and dim > 1:  # through the same sums as do
+            e = e + (bs * u * ny).abs() * ry * mean_abs * (C + 2 * r_ny)
+        out["dgate"] = (p.sum_to_size(gate.shape), e.sum_to_size(gate.shape))
+    return out
+
+
+def case(shape, dtype=BF, gate=None, post=True, pre=True, wtype=F32,
+         rs=1.0, bs=1.0, eps=1e-6, seed=0, use=("y", "h"), spread=1.0):
+    from baguanet import ops
+
+    gen = torch.Generator().manual_seed(seed)
+    rand = lambda s, t: torch.randn(s, generator=gen).to(t)
+    dim = shape[-1]
+    x, o = rand(shape, dtype), (rand(shape, F32) * spread).to(dtype)
+    g = None if gate is None else rand(gate, wtype)
+    wp = (1 + 0.2 * rand((dim,), F32)).to(wtype) if post else None
+    wn = (1 + 0.2 * rand((dim,), F32)).to(wtype) if pre else None
+    dy = rand(shape, dtype) if "y" in use else None
+    dh = rand(shape, dtype) if "h" in use and pre else None
+    dev = {k: None if v is None else v.cuda().requires_grad_()
+           for k, v in dict(x=x, branch=o, gate=g, post=wp, pre=wn).items()}
+    y, h = ops.gated_residual_norm(
+        dev["x"], dev["branch"], gate=dev["gate"], post_weight=dev["post"],
+        pre_weight=dev["pre"], residual_scale=rs, branch_scale=bs, eps=eps)
+    assert (h is None) == (not pre)
+    outs = [(v, d.cuda()) for v, d in ((y, dy), (h, dh)) if d is not None]
+    names = [k for k, v in dev.items() if v is not None]
+    grads = torch.autograd.grad([v for v, _ in outs], [dev[k] for k in names],
+                                [d for _, d in outs], allow_unused=True)
+    got = {"y": y, **({"h": h} if pre else {}),
+           **{"d" + k: v for k, v in zip(names, grads)}}
+    f32 = lambda v: float(torch.tensor(v, dtype=F32))
+    ref = reference(x, o, g, wp, wn, f32(rs), f32(bs), f32(eps), dy, dh,
+                    torch.finfo(dtype).eps / 2)
+    if dh is None and pre:
+        assert got.pop("dpre") is None
+    assert set(got) == set(ref)
+    for k, v in ref.items():
+        check(got[k], *v, what=k)
+
+
+@pytest.mark.parametrize("dim", [1, 2, 7, 64, 511, 512, 513, 1000, 1024, 1025,
+                                 2048, 2049, 4096, 4100, 8192, 8193, 16384,
+                                 16385, 32768])
+def test_widths(dim):
+    case((2, 5, dim), gate=(dim,), bs=0.5, seed=dim)
+    case((2, 5, dim), dtype=F32, gate=(2, 1, dim), bs=0.5, seed=dim + 1)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 9, 600, 4099])
+@pytest.mark.parametrize("dim", [72, 2080])
+def test_lengths(rows, dim):
+    case((rows, dim), gate=(dim,), seed=rows)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("own", [True, False])
+@pytest.mark.parametrize("dim", [136, 3000])
+def test_types(dtype, own, dim):
+    case((3, 17, dim), dtype=dtype, wtype=dtype if own else F32,
+         gate=(3, 1, dim), rs=0.7, bs=-1.3, eps=1e-5)
+
+
+@pytest.mark.parametrize("gate", [
+    None, (40,), (1, 1, 40), (6, 1, 40), (6, 23, 40), (6, 23, 1), (1, 23, 40),
+    (23, 40), (23, 1), (6, 1, 1), (1,), (), (1, 23, 1)])
+@pytest.mark.parametrize("post", [True, False])
+@pytest.mark.parametrize("pre", [True, False])
+def test_gates(gate, post, pre):
+    case((6, 23, 40), gate=gate, post=post, pre=pre, bs=0.3, dtype=F32)
+
+
+@pytest.mark.parametrize("shape,gate", [
+    ((700, 3, 264), (700, 1, 264)),    # more groups than workgroups
+    ((5, 1, 264), (5, 1, 264)),        # groups of one row
+    ((3, 1000, 264), (3, 1, 264)),     # groups cut in slices
+    ((2, 7, 33, 264), (2, 7, 1, 264)),
+    ((1500, 264), (1500, 1)),
+    ((3, 500, 2100), (3, 1, 2100)),
+    ((1, 1, 264), (1, 1, 264)),
+    ((1, 264), (1, 1)),
+])
+def test_groups(shape, gate):
+    case(shape, gate=gate, bs=0.5)
+
+
+@pytest.mark.parametrize("use", [("y",), ("h",)])
+@pytest.mark.parametrize("post", [True, False])
+def test_one_output_used(use, post):
+    case((4, 9, 520), gate=(520,), use=use, post=post)
+
+
+def test_small_values_keep_eps():
+    case((8, 256), dtype=F32, spread=1e-4, eps=1e-6, gate=(256,))
+
+
+def test_rms_norm():
+    from baguanet import ops
+
+    for dim in (5, 768, 5000):
+        for weight in (True, False):
+            gen = torch.Generator().manual_seed(dim)
+            x = torch.randn(11, dim, generator=gen).to(BF)
+            w = torch.randn(dim, generator=gen) if weight else None
+            dh = torch.randn(11, dim, generator=gen).to(BF)
+            xd = x.cuda().requires_grad_()
+            wd = w.cuda().requires_grad_() if weight else None
+            h = ops.rms_norm(xd, wd, eps=1e-5)
+            leaves = [xd] + ([wd] if weight else [])
+            grads = torch.autograd.grad(h, leaves, dh.cuda())
+            # x is read as it is: no half step of its type in the gradient
+            ref = reference(x, torch.zeros_like(x), None, None,
+                            w if weight else torch.ones(dim), 1.0, 1.0,
+                            float(torch.tensor(1e-5)), None, dh, 0.0)
+            check(h, *ref["h"], what="h")
+            check(grads[0], *ref["dx"], what="dx")
+            if weight:
+                check(grads[1], *ref["dpre"], what="dw")
+
+
+def test_empty():
+    from baguanet import ops
+
+    for shape in ((0, 16), (3, 0)):
+        x = torch.zeros(*shape, device="cuda", requires_grad=True)
+        w = torch.ones(shape[-1], device="cuda", requires_grad=True)
+        g = torch.ones(shape[-1], device="cuda", requires_grad=True)
+        y, h = ops.gated_residual_norm(x, x, g, w, w)
+        assert y.shape == h.shape == x.shape
+        grads = torch.autograd.grad((y.sum(), h.sum()), (x, w, g))
+        assert all((v == 0).all() for v in grads)
+
+
+def test_rows_do_not_mix():
+    """NaN and infinities of one row stay in it; a row of zeros is fine."""
+    from baguanet import ops
+
+    x = torch.randn(6, 300, device="cuda")
+    o = torch.randn(6, 300, device="cuda")
+    w = torch.ones(300, device="cuda")
+    y0, h0 = ops.gated_residual_norm(x, o, None, w, w)
+    x[1, 7], o[2, 3] = float("nan"), float("inf")
+    x[4], o[4] = 0, 0
+    y, h = ops.gated_residual_norm(x, o, None, w, w)
+    for r in (0, 3, 5):
+        assert torch.equal(y[r], y0[r]) and torch.equal(h[r], h0[r])
+    assert y[1, 7].isnan() and h[1].isnan().all()
+    assert h[2].isnan().any()
+    assert (y[4] == 0).all() and (h[4] == 0).all()
+
+
+def test_strides():
+    """Sliced, transposed and expanded inputs and gradients give what their
+    dense copies give."""
+    from baguanet import ops
+
+    gen = torch.Generator().manual_seed(2)
+    big = torch.randn(4, 10, 99, generator=gen).cuda()
+    w = torch.rand(128, generator=gen).cuda()[::2][:61]
+    pairs = [(big[..., 1:62], big[..., 30:91]),
+             (big[:, ::2, :61], big[:, 1::2, 5:66]),
+             (big[..., :61].transpose(0, 1), big[..., 7:68].transpose(0, 1)),
+             (big[:1, :1, :61].expand(4, 10, 61), big[..., 2:63]),
+             (big[..., :1].expand(4, 10, 61), big[..., 38:])]
+    for x, o in pairs:
+        for d in (big[..., :x.shape[-1]].reshape(-1)[:x.numel()].view(x.shape),
+                  x.detach() * 0.5, o[..., :1].expand_as(o)):
+            res = []
+            for dense in (False, True):
+                f = (lambda v: v.detach().clone(
+                    memory_format=torch.contiguous_format)) if dense else (
+                    lambda v: v.detach())
+                # a leaf for each use: autograd's own sum of three gradients
+                # of one leaf has no fixed order
+                leaves = [f(v).requires_grad_() for v in (x, o, w, w, w)]
+                y, h = ops.gated_residual_norm(*leaves)
+                res.append((y, h) + torch.autograd.grad(
+                    (y, h), leaves, (f(d), f(d))))
+            assert all(torch.equal(p, q) for p, q in zip(*res))
+
+
+def test_same_every_time():
+    from baguanet import ops
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    t = [torch.randn(3, 900, 520, device="cuda", generator=g).to(BF)
+         .requires_grad_() for _ in range(2)]
+    gate = torch.randn(3, 1, 520, device="cuda", generator=g).requires_grad_()
+    w = torch.rand(520, device="cuda", generator=g).requires_grad_()
+    first = None
+    for _ in range(4):
+        y, h = ops.gated_residual_norm(*t, gate, w, w)
+        out = torch.autograd.grad((y, h), (*t, gate, w), (t[0], t[1]))
+        first = first or out
+        assert all(torch.equal(a, b) for a, b in zip(out, first))
+
+
+def test_differences():
+    """Gradients against differences of the definition in 64 bits."""
+    from baguanet import ops
+
+    gen = torch.Generator().manual_seed(4)
+    shape, dim = (3, 5, 72), 72
+    vals = [torch.randn(*s, generator=gen) for s in
+            (shape, shape, (3, 1, dim), (dim,), (dim,))]
+    dirs = [torch.randn(*v.shape, generator=gen) for v in vals]
+    cy, ch = (torch.randn(*shape, generator=gen) for _ in range(2))
+    leaves = [v.cuda().requires_grad_() for v in vals]
+    y, h = ops.gated_residual_norm(*leaves, branch_scale=0.75, eps=1e-5)
+    grads = torch.autograd.grad((y, h), leaves, (cy.cuda(), ch.cuda()))
+
+    def f(s):
+        x, o, g, wp, wn = (v.double() + s * d.double()
+                           for v, d in zip(vals, dirs))
+        n = lambda v: v / (v.pow(2).mean(-1, keepdim=True) + 1e-5).sqrt()
+        y = x + 0.75 * g * n(o) * wp
+        return (y * cy).sum() + (n(y) * wn * ch).sum()
+
+    # central differences of two steps cancel the h**2 term; what is left is
+    # of the order of h**4 = 1e-12 and rounding of 1e-16 * |f| / h
+    h1 = 1e-3
+    slope = (8 * (f(h1) - f(-h1)) - (f(2 * h1) - f(-2 * h1))) / (12 * h1)
+    ref = reference(*vals, 1.0, 0.75, float(torch.tensor(1e-5)), cy, ch, U)
+    got = bound = 0.0
+    for name, d, v in zip(("dx", "dbranch", "dgate", "dpost", "dpre"),
+                          dirs, grads):
+        r, e = ref[name]
+        got = got + (v.double().cpu() * d).sum()
+        bound = bound + ((e + r.abs() * U) * d.abs()).sum()
+    assert (got - slope).abs() <= bound + 1e-7 * slope.abs() + 1e-7
+
+
+def test_not_twice_differentiable():
+    from baguanet import ops
+
+    x = torch.randn(3, 8, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(ops.rms_norm(x).sum(), x, create_graph=True)
+
+
+def test_other_stream_and_graph():
+    from baguanet import ops
+
+    x, o = (torch.randn(4, 300, 1100, device="cuda").to(BF).requires_grad_()
+            for _ in range(2))
+    gate = torch.randn(4, 1, 1100, device="cuda").requires_grad_()
+    w = torch.rand(1100, device="cuda").requires_grad_()
+    dy, dh = torch.randn_like(x), torch.randn_like(x)
+
+    def step():
+        y, h = ops.gated_residual_norm(x, o, gate, w, w, branch_scale=0.1)
+        return (y.detach(), h.detach()) + torch.autograd.grad(
+            (y, h), (x, o, gate, w), (dy, dh))
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(4):
+        with torch.no_grad():
+            for t in (x, o, gate, dy, dh):
+                t.normal_()
+            w.uniform_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))

@@ -1,0 +1,90 @@
+"""Wrong calls of the training-step operators are refused before anything
+runs, the same way with and without a GPU."""
+
+import pytest
+import torch
+
+from baguanet import ops
+
+
+def _bf(*shape):
+    return torch.zeros(*shape, dtype=torch.bfloat16)
+
+
+TOK = torch.zeros(3, dtype=torch.int64)
+
+
+@pytest.mark.parametrize("call,what", [
+    (lambda: ops.embedding(_bf(4), TOK), r"weight must be \[vocab, dim\]"),
+    (lambda: ops.embedding(torch.zeros(4, 8, dtype=torch.float64), TOK),
+     "weight must be float32, bfloat16 or float16"),
+    (lambda: ops.embedding(_bf(4, 8), TOK.float()), "int64 or int32"),
+    (lambda: ops.embedding(_bf(4, 8), TOK, padding_idx=4), "padding_idx 4"),
+    (lambda: ops.embedding(_bf(4, 8), TOK, padding_idx=-5), "padding_idx -5"),
+    (lambda: ops.embedding(_bf(4, 8), TOK, out_dtype=torch.int32),
+     "out_dtype"),
+    (lambda: ops.embedding(_bf(4, 8), TOK), "weight must be on the GPU"),
+    (lambda: ops.rms_norm(torch.zeros((), dtype=torch.float32)), "scalar"),
+    (lambda: ops.rms_norm(torch.zeros(4, 8, dtype=torch.int32)), "x must be"),
+    (lambda: ops.rms_norm(_bf(4, 8), _bf(9)), r"weight must be \[8\]"),
+    (lambda: ops.rms_norm(_bf(4, 8), torch.zeros(8, dtype=torch.float16)),
+     "float32 or of x's type"),
+    (lambda: ops.rms_norm(_bf(2, 32769)), "at most 32768 columns"),
+    (lambda: ops.rms_norm(_bf(4, 8), eps=-1.0), "eps"),
+    (lambda: ops.rms_norm(_bf(4, 8)), "x must be on the GPU"),
+    (lambda: ops.gated_residual_norm(_bf(4, 8), _bf(4, 9)), "x's shape"),
+    (lambda: ops.gated_residual_norm(_bf(4, 8), torch.zeros(4, 8)),
+     "x's type"),
+    (lambda: ops.gated_residual_norm(_bf(4, 8), _bf(4, 8), gate=_bf(3, 8)),
+     "cannot be broadcast"),
+    (lambda: ops.gated_residual_norm(_bf(4, 8), _bf(4, 8),
+                                     gate=_bf(1, 4, 8)),
+     "cannot be broadcast"),
+    (lambda: ops.gated_residual_norm(
+        _bf(4, 8), _bf(4, 8), gate=torch.zeros(8, dtype=torch.float16)),
+     "gate must be float32 or of x's type"),
+    (lambda: ops.gated_residual_norm(_bf(4, 8), _bf(4, 8),
+                                     post_weight=_bf(7)),
+     r"post_weight must be \[8\]"),
+    (lambda: ops.gated_residual_norm(_bf(4, 8), _bf(4, 8),
+                                     pre_weight=_bf(1, 8)),
+     r"pre_weight must be \[8\]"),
+    (lambda: ops.gated_residual_norm(_bf(4, 8), _bf(4, 8)),
+     "x must be on the GPU"),
+    (lambda: ops.act8_pack(torch.zeros(4, 8, dtype=torch.float64)),
+     "x must be"),
+    (lambda: ops.act8_pack(_bf(4, 8)), "x must be on the GPU"),
+    (lambda: ops.linear_act8(_bf(4, 8), _bf(5, 9)), r"\[out, 8\]"),
+    (lambda: ops.linear_act8(_bf(4, 8), torch.zeros(5, 8)), "x's type"),
+    (lambda: ops.linear_act8(_bf(4, 8), _bf(5, 8), _bf(4)),
+     r"bias must be \[5\]"),
+    (lambda: ops.linear_act8(_bf(4, 8), _bf(5, 8)), "on the GPU"),
+    (lambda: ops.silu_mul_act8(_bf(4, 7)), "two halves"),
+    (lambda: ops.silu_mul_act8(_bf(4, 8)), "on the GPU"),
+])
+def test_refused(call, what):
+    with pytest.raises(RuntimeError, match=what):
+        call()
+
+
+def _kept(rows=4, cols=40, pitch=64, groups=2, dtype=torch.bfloat16):
+    return ops.Act8(torch.zeros(rows, pitch, dtype=torch.uint8),
+                    torch.zeros(rows, groups, dtype=torch.uint8),
+                    torch.Size((rows, cols)), dtype)
+
+
+@pytest.mark.parametrize("call,what", [
+    (lambda: ops.act8_unpack(_kept(pitch=40)), "codes must be"),
+    (lambda: ops.act8_unpack(_kept(groups=3)), "exponents must be"),
+    (lambda: ops.act8_unpack(_kept(dtype=torch.int32)), "dtype must be"),
+    (lambda: ops.act8_unpack(_kept()), "codes must be on the GPU"),
+    (lambda: ops.act8_wgrad(_bf(5, 8), _kept()), "rows of the kept input"),
+    (lambda: ops.act8_wgrad(_bf(2, 2, 8), _kept()), "rows of the kept input"),
+    (lambda: ops.act8_wgrad(torch.zeros(4, 8), _kept()),
+     "the kept input's type"),
+    (lambda: ops.act8_wgrad(_bf(4, 8), _kept(pitch=96)), "codes must be"),
+    (lambda: ops.act8_wgrad(_bf(4, 8), _kept()), "dy must be on the GPU"),
+])
+def test_kept_refused(call, what):
+    with pytest.raises(RuntimeError, match=what):
+        call()
