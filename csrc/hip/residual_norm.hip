@@ -19,7 +19,9 @@
 // registers too, over a slice of rows for each workgroup, and are joined by a
 // second small kernel in a fixed order: no atomics, the same result in every
 // run.  All sums and products are in fp32; y and h are rounded once, and h
-// is taken from y before its rounding.
+// is taken from y before its rounding.  The backward pass reads x and o, which
+// costs what reading y and o would, and computes y again: from a rounded y
+// the weights' fp32 gradients would be no better than the activations' type.
 #include <hip/hip_runtime.h>
 
 #include "device_types.h"
@@ -159,7 +161,7 @@ template <typename T, int TPR, int VPT>
 __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
     NormBwd a, Cut cut, Parts parts) {
   constexpr int kTeams = block_of<TPR>() / TPR;
-  __shared__ float red[2][4 * (TPR / kWave)];
+  __shared__ float red[2][3 * (TPR / kWave)];
   // the teams' column sums on their way to the first team
   __shared__ float joint[kTeams > 1 ? kTeams - 1 : 1]
                         [kTeams > 1 ? TPR * VPT * kVec : 1];
@@ -224,13 +226,13 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
       for (int j = 0; j < VPT; j++)
         gate[j] = weight_upto<T>(a.gate, a.gate32, grp * a.dim + col[j], m[j]);
     }
-    typename RowVec<T>::type yn[VPT], on[VPT], dyn[VPT], dhn[VPT];
+    typename RowVec<T>::type xn[VPT], on[VPT], dyn[VPT], dhn[VPT];
     float ro_n = 1.f, ry_n = 0.f, g_n = 1.f;
     auto fetch = [&](int64_t r) {
 #pragma unroll
       for (int j = 0; j < VPT; j++) {
         if (a.dh) {
-          yn[j] = raw_upto((const T*)a.y + r * a.ystride + col[j], m[j]);
+          xn[j] = raw_upto((const T*)a.x + r * a.xstride + col[j], m[j]);
           dhn[j] = raw_upto((const T*)a.dh + r * a.dhstride + col[j], m[j]);
         }
         if (a.dy)
@@ -248,40 +250,44 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
     if (row < last) fetch(row);
     for (; row < last; row += kTeams) {
       const float ry = ry_n, ro = ro_n, g_row = g_n;
-      float8 dY[VPT], no[VPT], ny[VPT], t[VPT], g[VPT];
+      float8 dY[VPT], no[VPT], ny[VPT], g[VPT];
       // sums: ny * t;  q * (dy + ry * t);  q * ny, with q = no * post * gate:
       // the mean that do needs then follows without a second pass.
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < VPT; j++) {
-        ny[j] = t[j] = dY[j] = 0.f;
-        if (a.dy) dY[j] = widen(dyn[j]);
-        if (a.dh) {
-          const float8 dh = widen(dhn[j]);
-          ny[j] = widen(yn[j]) * ry;
-          t[j] = dh * pre[j];
-          acc_pre[j] += dh * ny[j];
-          dY[j] += t[j] * ry;
-          s[0] += sum8(ny[j] * t[j]);
-        }
+        ny[j] = dY[j] = 0.f;
+        float8 c;
         if (a.branch) {
           no[j] = widen(on[j]) * ro;
           g[j] = gate[j] * g_row;
           if (a.gmode == Gate::kFull)
             g[j] = weight_upto<T>(a.gate, a.gate32, row * a.dim + col[j], m[j]);
-          const float8 q = no[j] * post[j] * gate[j];
-          const float8 f = a.gmode == Gate::kFull ? q * g[j] : q;
-          s[1] += sum8(f * dY[j]);
-          s[2] += sum8(f * ny[j]);
+          c = no[j] * post[j];
+        }
+        if (a.dy) dY[j] = widen(dyn[j]);
+        if (a.dh) {
+          const float8 dh = widen(dhn[j]);
+          float8 y = widen(xn[j]) * a.residual_scale;
+          if (a.branch) y += c * g[j] * a.branch_scale;
+          ny[j] = y * ry;
+          const float8 t = dh * pre[j];
+          acc_pre[j] += dh * ny[j];
+          dY[j] += t * ry;
+          s[0] += sum8(ny[j] * t);
+        }
+        if (a.branch) {
+          const float8 q = c * (a.gmode == Gate::kFull ? g[j] : gate[j]);
+          s[1] += sum8(q * dY[j]);
+          s[2] += sum8(q * ny[j]);
         }
       }
       if (row + kTeams < last) fetch(row + kTeams);
-      float v[3] = {s[0], s[1], s[2]};
-      row_sums<TPR>(v, red[parity]);
+      row_sums<TPR>(s, red[parity]);
       parity ^= 1;
-      const float k0 = ry * v[0] * inv_dim;
+      const float k0 = ry * s[0] * inv_dim;
       // sum of no * post * gate * dY, without the row's own gate
-      const float sq = v[1] - k0 * v[2];
+      const float sq = s[1] - k0 * s[2];
       const float k1 = sq * a.branch_scale * g_row * inv_dim;
       if (a.gmode == Gate::kRow && a.dgate && lane == 0) {
         const float dg = sq * a.branch_scale;

@@ -67,8 +67,8 @@ struct NormFwd {
 hipError_t norm_forward(const NormFwd& a, hipStream_t stream);
 
 struct NormBwd {
-  const void* y;       // [rows, dim], rows `ystride` apart
-  const void* branch;  // as in the forward pass
+  const void* x;       // [rows, dim] and branch, as in the forward pass: y is
+  const void* branch;  // computed again, for its unrounded value
   const void* gate;
   const void* post;
   const void* pre;
@@ -82,7 +82,7 @@ struct NormBwd {
   void* dpost;         // [dim], or null
   void* dpre;          // [dim], or null
   void* workspace;     // norm_workspace() bytes
-  int64_t rows, dim, ystride, bstride, dystride, dhstride;
+  int64_t rows, dim, xstride, bstride, dystride, dhstride;
   int64_t group_rows;
   float residual_scale, branch_scale;
   Gate gmode;

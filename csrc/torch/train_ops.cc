@@ -248,7 +248,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
     }
     check_launch(norm_forward(a, stream_of(x)), "residual norm");
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({branch.defined() ? y : want_h ? xr.t : Tensor(),
+    ctx->save_for_backward({want_h ? xr.t : Tensor(),
                             branch.defined() ? br.t : Tensor(), gate, post,
                             pre, rbranch, ry});
     ctx->saved_data["scales"] =
@@ -268,7 +268,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
     no_double_backward("residual norm");
     variable_list out(11);
     const auto saved = ctx->get_saved_variables();
-    const Tensor &y = saved[0], &branch = saved[1], &gate = saved[2],
+    const Tensor &x = saved[0], &branch = saved[1], &gate = saved[2],
                  &post = saved[3], &pre = saved[4], &rbranch = saved[5],
                  &ry = saved[6];
     Tensor dy, dh;
@@ -292,7 +292,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
     a.branch_scale = (float)scales[1];
     a.gmode = (Gate)g[0];
     a.group_rows = g[1];
-    Rows yr, br, dyr, dhr;
+    Rows xr, br, dyr, dhr;
     Tensor dx = at::empty(some.sizes(), some.options());
     a.dx = dx.data_ptr();
     Tensor dbranch, dgate, dpost, dpre;
@@ -302,10 +302,10 @@ struct NormFn : torch::autograd::Function<NormFn> {
       a.dystride = dyr.stride;
     }
     if (dh.defined()) {
-      yr = as_rows(y);
+      xr = as_rows(x);
       dhr = as_rows(dh);
-      a.y = yr.t.data_ptr();
-      a.ystride = yr.stride;
+      a.x = xr.t.data_ptr();
+      a.xstride = xr.stride;
       a.dh = dhr.t.data_ptr();
       a.dhstride = dhr.stride;
       a.ry = ry.data_ptr<float>();

@@ -6,9 +6,8 @@ the value, and half of float16's smallest step of 2**-24).  Before that all is
 fp32: a sum of at most 32768 terms goes through fewer than 48 additions on any
 path (8 of a vector, 4 vectors, 6 lane exchanges, 16 waves), and the products
 around it add fewer than 16 roundings, so C = 64 half steps of 2**-24, relative
-to the sum of the magnitudes, bound each number before its last rounding.  The
-backward pass reads y as it was rounded, so what it takes from y carries half
-a step of the type more.  Sums over R rows add R roundings.
+to the sum of the magnitudes, bound each number before its last rounding.
+Sums over R rows add R roundings.
 """
 
 import pytest
@@ -31,11 +30,8 @@ def check(got, ref, extra, what):
     assert (off <= tol).all(), (what, (off / tol).max().item())
 
 
-def reference(x, o, gate, post, pre, rs, bs, eps, dy, dh, half):
-    """Values, gradients and how far each may be off before its rounding.
-
-    `half`: half a step of the activations' type, relative.
-    """
+def reference(x, o, gate, post, pre, rs, bs, eps, dy, dh):
+    """Values, gradients and how far each may be off before its rounding."""
     dim = x.shape[-1]
     x, o = x.double(), o.double()
     one = torch.ones((), dtype=torch.float64)
@@ -61,14 +57,14 @@ def reference(x, o, gate, post, pre, rs, bs, eps, dy, dh, half):
     if pre is not None and dh is not None:
         dh = dh.double()
         t = dh * wn
-    # relative errors of ny as the backward pass has it
     rel = (y.abs() * e_y).mean(-1, keepdim=True) * ry ** 2
-    r_ny = half + C + rel
+    e_ny = ry * e_y + ny.abs() * (C + rel)
     mean = (ny * t).mean(-1, keepdim=True)
     mean_abs = (ny * t).abs().mean(-1, keepdim=True)
+    e_mean = (e_ny * t.abs()).mean(-1, keepdim=True) + C * mean_abs
     d = dy + ry * (t - ny * mean)
     d_abs = dy.abs() + ry * (t.abs() + ny.abs() * mean_abs)
-    e_d = (C + rel) * d_abs + 2 * ry * ny.abs() * mean_abs * r_ny
+    e_d = (C + rel) * d_abs + ry * (e_ny * mean_abs + ny.abs() * e_mean)
     out["dx"] = (rs * d, abs(rs) * e_d)
     c = bs * g * wp
     if post is None:
@@ -77,9 +73,6 @@ def reference(x, o, gate, post, pre, rs, bs, eps, dy, dh, half):
         mean = (no * c * d).mean(-1, keepdim=True)
         e_in = (e_d + C * d_abs) * c.abs()
         e_mean = (no.abs() * e_in).mean(-1, keepdim=True)
-        # the kernel's mean is a difference of two sums of these magnitudes
-        e_mean = e_mean + (ny * no * c).abs().mean(-1, keepdim=True) * (
-            ry * mean_abs * (C + 2 * r_ny))
         out["dbranch"] = (ro * (c * d - no * mean),
                           ro * (e_in + no.abs() * (e_mean + C * mean.abs())))
     rows = x.numel() // dim
@@ -87,7 +80,7 @@ def reference(x, o, gate, post, pre, rs, bs, eps, dy, dh, half):
     if pre is not None and dh is not None:
         p = dh * ny
         out["dpre"] = (flat(p).sum(0),
-                       flat(p.abs() * (r_ny + C + rows * U)).sum(0))
+                       flat(dh.abs() * e_ny + p.abs() * (C + rows * U)).sum(0))
     if post is not None:
         p = bs * g * d * no
         e = (bs * g * no).abs() * (e_d + (C + rows * U) * d_abs)
@@ -95,8 +88,6 @@ def reference(x, o, gate, post, pre, rs, bs, eps, dy, dh, half):
     if gate is not None:
         p = bs * d * u
         e = (bs * u).abs() * (e_d + (C + (rows + dim) * U) * d_abs)
-        if gate.shape[-1:] == (1,) and dim > 1:  # through the same sums as do
-            e = e + (bs * u * ny).abs() * ry * mean_abs * (C + 2 * r_ny)
         out["dgate"] = (p.sum_to_size(gate.shape), e.sum_to_size(gate.shape))
     return out
 
@@ -127,8 +118,7 @@ def case(shape, dtype=BF, gate=None, post=True, pre=True, wtype=F32,
     got = {"y": y, **({"h": h} if pre else {}),
            **{"d" + k: v for k, v in zip(names, grads)}}
     f32 = lambda v: float(torch.tensor(v, dtype=F32))
-    ref = reference(x, o, g, wp, wn, f32(rs), f32(bs), f32(eps), dy, dh,
-                    torch.finfo(dtype).eps / 2)
+    ref = reference(x, o, g, wp, wn, f32(rs), f32(bs), f32(eps), dy, dh)
     if dh is None and pre:
         assert got.pop("dpre") is None
     assert set(got) == set(ref)
@@ -205,10 +195,9 @@ def test_rms_norm():
             h = ops.rms_norm(xd, wd, eps=1e-5)
             leaves = [xd] + ([wd] if weight else [])
             grads = torch.autograd.grad(h, leaves, dh.cuda())
-            # x is read as it is: no half step of its type in the gradient
             ref = reference(x, torch.zeros_like(x), None, None,
                             w if weight else torch.ones(dim), 1.0, 1.0,
-                            float(torch.tensor(1e-5)), None, dh, 0.0)
+                            float(torch.tensor(1e-5)), None, dh)
             check(h, *ref["h"], what="h")
             check(grads[0], *ref["dx"], what="dx")
             if weight:
@@ -317,7 +306,7 @@ def test_differences():
     # of the order of h**4 = 1e-12 and rounding of 1e-16 * |f| / h
     h1 = 1e-3
     slope = (8 * (f(h1) - f(-h1)) - (f(2 * h1) - f(-2 * h1))) / (12 * h1)
-    ref = reference(*vals, 1.0, 0.75, float(torch.tensor(1e-5)), cy, ch, U)
+    ref = reference(*vals, 1.0, 0.75, float(torch.tensor(1e-5)), cy, ch)
     got = bound = 0.0
     for name, d, v in zip(("dx", "dbranch", "dgate", "dpost", "dpre"),
                           dirs, grads):
