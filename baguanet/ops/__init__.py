@@ -108,7 +108,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     """``x / sqrt(mean(x ** 2) + eps) * weight`` over the last dimension.
 
     ``weight`` is ``[dim]``, float32 or of x's type; ``dim`` is at most
-    32768.  This is the norm before a network's first block; those between
+    16384.  This is the norm before a network's first block; those between
     blocks are part of :func:`gated_residual_norm`.
     """
     return _load().rms_norm(x, weight, eps)
@@ -128,7 +128,7 @@ def gated_residual_norm(x: torch.Tensor, branch: torch.Tensor,
         h = rms_norm(y, pre_weight)                (None, without a weight)
 
     Returns ``(y, h)``: the residual stream and the next block's input.
-    ``x`` and ``branch`` have one shape and type, with at most 32768 columns.
+    ``x`` and ``branch`` have one shape and type, with at most 16384 columns.
     ``gate`` may be anything that broadcasts to x: ``[dim]`` for each column,
     ``[batch, 1, dim]`` for each sequence's columns, ``[batch, length, 1]``
     for each row, or one value for each element.  It and the weights are

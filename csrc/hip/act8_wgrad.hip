@@ -27,9 +27,9 @@ typedef __attribute__((address_space(3))) short4v* LdsShort4;
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef fp16 fp16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kThreads = 256;     // four waves, two by two
-constexpr int kTN = 128, kTK = 128;  // of dW for a workgroup
-constexpr int kTM = 32;           // rows summed for each tile in LDS
+constexpr int kThreads = 256;  // four waves, two by two
+constexpr int kTM = 64;         // rows summed for each tile in LDS
+constexpr int kSteps = kTM / 16;  // of the matrix instructions for a tile
 
 template <typename T>
 __device__ inline float16v mfma(short8v a, short8v b, float16v c);
@@ -46,124 +46,251 @@ __device__ inline float16v mfma<fp16>(short8v a, short8v b, float16v c) {
       0);
 }
 
-// A tile in LDS: kTM rows of `width` 16-bit values.  Four rows that one
+// Two codes' values, exact in bf16 and fp16.
+template <typename T>
+__device__ inline uint32_t widen2(uint32_t codes, float scale, bool high);
+template <>
+__device__ inline uint32_t widen2<bf16>(uint32_t codes, float scale,
+                                        bool high) {
+  return __builtin_bit_cast(
+      uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale,
+                                                                 true)
+                     : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale,
+                                                                 false));
+}
+template <>
+__device__ inline uint32_t widen2<fp16>(uint32_t codes, float scale,
+                                        bool high) {
+  return __builtin_bit_cast(
+      uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale,
+                                                                true)
+                     : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale,
+                                                                false));
+}
+
+// A tile in LDS: kTM rows of kWidth 16-bit values.  Four rows that one
 // transposing read takes together lie on different banks: the 64-byte
 // blocks of a row are exchanged by the row's last two bits.
 template <int kWidth>
 __device__ inline int lds_at(int row, int col) {
-  const int block = (col >> 5) ^ (row & 3);
-  return row * kWidth + (block << 5) + (col & 31);
+  return row * kWidth + (((col >> 5) ^ (row & 3)) << 5) + (col & 31);
 }
 
-// 8 rows of one column for each lane: lanes 0..31 take the columns col0..+31
-// of rows row0..+7, the others those of rows row0 + 8..+15.
+// 8 rows of one column for each lane, from `p`, the lane's place for the
+// fragment's first row: lanes 0..31 take 32 columns of the rows 0..7, the
+// others those of the rows 8..15.
 template <int kWidth>
-__device__ inline short8v read_fragment(const short* tile, int row0,
-                                        int col0) {
-  const int lane = threadIdx.x % kWave;
-  const int row = row0 + (lane / 32) * 8 + (lane % 16) / 4;
-  const int col = col0 + (lane / 16 % 2) * 16 + (lane % 4) * 4;
-  const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (LdsShort4)(tile + lds_at<kWidth>(row, col)));
-  const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (LdsShort4)(tile + lds_at<kWidth>(row + 4, col)));
+__device__ inline short8v read_fragment(const short* p) {
+  const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)p);
+  const short4v hi =
+      __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)(p + 4 * kWidth));
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// One product's shape: `planes` row blocks of `m` rows in dy, one in x'.
+// Memory that is read a tile of rows at a time.  Reads behind its end give
+// zeros (the hardware checks them against the descriptor's size), so the
+// last tile needs no conditions; those behind a row's end give the next
+// row's values, which only reach columns that are not written.
+struct Stream {
+  const char* base;
+  int64_t bytes;      // in all
+  int64_t tile;       // from one tile to the next
+};
+
+__device__ inline __amdgpu_buffer_rsrc_t at_tile(const Stream& s, int64_t t) {
+  int64_t left = s.bytes - t * s.tile;
+  left = left < 0 ? 0 : left > INT32_MAX ? INT32_MAX : left;
+  const char* p = s.base + (left ? t * s.tile : 0);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)left, 0x00027000);
+}
+
+// One product: dy in tiles of kTM rows, `tiles` in all; x' starts again
+// after `xtiles` of them (the planes of an fp32 gradient).
 struct Product {
-  const void* dy;
-  int64_t dstride, plane;  // elements between rows and between planes
-  int planes, slices;
-  int64_t slice_rows;      // of the planes * m rows, a multiple of kTM
+  Stream dy, codes, exps;
+  int dpitch, cpitch;      // bytes between rows of dy and of codes
+  int tiles, xtiles;
+  int slices, slice_tiles;
+  int ntiles, ktiles;
+  int64_t n, k;
+  void* dw;
   float* partial;          // [slices, n, k] where slices > 1
 };
 
-// T: bf16 or fp16, the operands' type.  O: the type of dW.
-template <typename T, typename O>
-__global__ __launch_bounds__(kThreads) void act8_wgrad_kernel(Act8Wgrad a,
-                                                              Product p) {
-  __shared__ __attribute__((aligned(16))) short sy[kTM * kTN];
-  __shared__ __attribute__((aligned(16))) short sx[kTM * kTK];
-  const int64_t n0 = (int64_t)blockIdx.x * kTN, k0 = (int64_t)blockIdx.y * kTK;
+// The workgroup's tile of dW.  Workgroups go to the 8 XCDs in turn; each XCD
+// takes a run of tiles, in strips 8 tiles high, so that those at work
+// together read the same parts of dy and x' through its L2.
+__device__ inline void pick_tile(const Product& p, int& tn, int& tk) {
+  const int total = p.ntiles * p.ktiles, id = blockIdx.x;
+  const int xcd = id % 8, each = total / 8, more = total % 8;
+  const int at = xcd * each + (xcd < more ? xcd : more) + id / 8;
+  const int strip = at / (8 * p.ktiles), in = at % (8 * p.ktiles);
+  const int high = p.ntiles - strip * 8 < 8 ? p.ntiles - strip * 8 : 8;
+  tn = strip * 8 + in % high;
+  tk = in / high;
+}
+
+// T: bf16 or fp16, the operands' type.  O: the type of dW.  A wave computes
+// FN by FK blocks of 32 by 32.
+//
+// Two tiles are in LDS: the matrix instructions of one overlap with the
+// writing of the next, whose rows are in registers by then, and with the
+// loads of the one after.  A step's fragments are read during the step
+// before, across the tiles' border too: the one barrier of a tile stands
+// before its last step, when all its fragments have been read and all of the
+// next tile is written.
+template <typename T, typename O, int FN, int FK>
+__global__ __launch_bounds__(kThreads, FN * FK > 8 ? 1 : 2)
+void act8_wgrad_kernel(Product p) {
+  constexpr int kTN = 64 * FN, kTK = 64 * FK;
+  constexpr int kPassN = kTM * kTN / 8 / kThreads;
+  constexpr int kPassK = kTM * kTK / 8 / kThreads;
+  constexpr int kRowsN = kTM / kPassN, kRowsK = kTM / kPassK;  // of a pass
+  constexpr int kTile = kTM * (kTN + kTK);  // both operands' tiles
+  __shared__ __attribute__((aligned(16))) short lds[2 * kTile];
+  int tn, tk;
+  pick_tile(p, tn, tk);
+  const int64_t n0 = (int64_t)tn * kTN, k0 = (int64_t)tk * kTK;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int wn = (wave / 2) * (kTN / 2), wk = (wave % 2) * (kTK / 2);
-  const int64_t total = p.planes * a.m;
-  const int64_t begin = blockIdx.z * p.slice_rows;
-  const int64_t end =
-      begin + p.slice_rows < total ? begin + p.slice_rows : total;
+  const int t0 = blockIdx.y * p.slice_tiles;
+  const int t1 = t0 + p.slice_tiles < p.tiles ? t0 + p.slice_tiles : p.tiles;
 
-  float16v acc[2][2];
+  // global: this thread's 8 columns of a row of a pass
+  const int ry = threadIdx.x / (kTN / 8), cy = threadIdx.x % (kTN / 8) * 8;
+  const int rx = threadIdx.x / (kTK / 8), cx = threadIdx.x % (kTK / 8) * 8;
+  const int gy = ry * p.dpitch + (int)(n0 + cy) * 2;
+  const int gx = rx * p.cpitch + (int)(k0 + cx);
+  // LDS: rows of a pass are kRows apart, a multiple of 4
+  const int ly = lds_at<kTN>(ry, cy);
+  const int lx = kTM * kTN + lds_at<kTK>(rx, cx);
+  // fragments: the lane's place in each, for the tile's first row
+  const int fr = (lane / 32) * 8 + (lane % 16) / 4;
+  const int fc = (lane / 16 % 2) * 16 + (lane % 4) * 4;
+  int fy[FN], fx[FK];
 #pragma unroll
-  for (int i = 0; i < 2; i++)
+  for (int i = 0; i < FN; i++) fy[i] = lds_at<kTN>(fr, wn + i * 32 + fc);
 #pragma unroll
-    for (int j = 0; j < 2; j++) acc[i][j] = 0.f;
+  for (int i = 0; i < FK; i++) 
+    fx[i] = kTM * kTN + lds_at<kTK>(fr, wk + i * 32 + fc);
 
-  for (int64_t m0 = begin; m0 < end; m0 += kTM) {
-    // dy: 16 lanes to a row of 128, two rows for each lane
+  typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+  typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+  uint4v hy[kPassN];
+  uint2v hx[kPassK];
+  uint32_t he[kPassK];
+  __amdgpu_buffer_rsrc_t by, bx, be;
+  auto aim = [&](int t) {  // the descriptors at tile t, past the end: empty
+    by = at_tile(p.dy, t < t1 ? t : INT32_MAX);
+    const int tx = t < t1 ? t % p.xtiles : INT32_MAX;
+    bx = at_tile(p.codes, tx);
+    be = at_tile(p.exps, tx);
+  };
+  auto load_y = [&](int i) {
+    hy[i] = __builtin_amdgcn_raw_buffer_load_b128(by, gy,
+                                                  i * kRowsN * p.dpitch, 0);
+  };
+  auto load_x = [&](int i) {
+    const int off = i * kRowsK * p.cpitch;
+    hx[i] = __builtin_amdgcn_raw_buffer_load_b64(bx, gx, off, 0);
+    he[i] = __builtin_amdgcn_raw_buffer_load_b8(be, gx >> 5, off >> 5, 0);
+  };
+  auto write_y = [&](int buf, int i) {
+    *(uint4v*)&lds[buf + ly + i * kRowsN * kTN] = hy[i];
+  };
+  auto write_x = [&](int buf, int i) {
+    const float scale = __uint_as_float(he[i] << 23);
+    uint4v v;
+    v[0] = widen2<T>(hx[i][0], scale, false);
+    v[1] = widen2<T>(hx[i][0], scale, true);
+    v[2] = widen2<T>(hx[i][1], scale, false);
+    v[3] = widen2<T>(hx[i][1], scale, true);
+    *(uint4v*)&lds[buf + lx + i * kRowsK * kTK] = v;
+  };
+
+  float16v acc[FN][FK];
 #pragma unroll
-    for (int i = 0; i < kTM * kTN / (kThreads * 8); i++) {
-      const int at = i * kThreads + threadIdx.x;
-      const int r = at / (kTN / 8), c = at % (kTN / 8) * 8;
-      typename RowVec<T>::type v = (T)0.f;
-      const int64_t row = m0 + r, left = a.n - n0 - c;
-      if (row < end && left > 0) {
-        const int64_t pl = row / a.m, rr = row % a.m;
-        v = raw_upto((const T*)p.dy + pl * p.plane + rr * p.dstride + n0 + c,
-                     left < 8 ? (int)left : 8);
-      }
-      *(typename RowVec<T>::type*)&sy[lds_at<kTN>(r, c)] = v;
+  for (int i = 0; i < FN; i++)
+#pragma unroll
+    for (int j = 0; j < FK; j++) acc[i][j] = 0.f;
+  short8v ay[2][FN], ax[2][FK];
+  auto read_step = [&](int buf, int step, int to) {
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+      ay[to][i] = read_fragment<kTN>(&lds[buf + fy[i] + step * 16 * kTN]);
+#pragma unroll
+    for (int i = 0; i < FK; i++)
+      ax[to][i] = read_fragment<kTK>(&lds[buf + fx[i] + step * 16 * kTK]);
+  };
+
+  aim(t0);
+#pragma unroll
+  for (int i = 0; i < kPassN; i++) load_y(i);
+#pragma unroll
+  for (int i = 0; i < kPassK; i++) load_x(i);
+  aim(t0 + 1);
+#pragma unroll
+  for (int i = 0; i < kPassN; i++) {
+    write_y(0, i);
+    load_y(i);
+  }
+#pragma unroll
+  for (int i = 0; i < kPassK; i++) {
+    write_x(0, i);
+    load_x(i);
+  }
+  __syncthreads();
+  read_step(0, 0, 0);
+
+  int cur = 0;  // where in LDS the tile at work begins
+  for (int t = t0; t < t1; t++) {
+    const int nxt = kTile - cur;
+    aim(t + 2);
+#pragma unroll
+    for (int s = 0; s < kSteps; s++) {
+      if (s == kSteps - 1) __syncthreads();
+      read_step(s == kSteps - 1 ? nxt : cur, (s + 1) % kSteps, (s + 1) % 2);
+      // the next tile's rows into LDS, spread over the steps but the last
+#pragma unroll
+      for (int i = 0; i < kPassN; i++)
+        if (i * (kSteps - 1) / kPassN == s) {
+          write_y(nxt, i);
+          load_y(i);
+        }
+#pragma unroll
+      for (int i = 0; i < kPassK; i++)
+        if (i * (kSteps - 1) / kPassK == s) {
+          write_x(nxt, i);
+          load_x(i);
+        }
+#pragma unroll
+      for (int i = 0; i < FN; i++)
+#pragma unroll
+        for (int j = 0; j < FK; j++)
+          acc[i][j] = mfma<T>(ay[s % 2][i], ax[s % 2][j], acc[i][j]);
     }
-    // x': 16 lanes to a row too
-#pragma unroll
-    for (int i = 0; i < kTM * kTK / (kThreads * 8); i++) {
-      const int at = i * kThreads + threadIdx.x;
-      const int r = at / (kTK / 8), c = at % (kTK / 8) * 8;
-      float8 v = 0.f;
-      const int64_t row = m0 + r;
-      if (row < end && k0 + c < a.pitch) {
-        const int64_t at8 = row % a.m * a.pitch + k0 + c;
-        v = decode8(*(const uint2*)(a.codes + at8),
-                    a.exps[at8 / kAct8Group] - 127);
-      }
-      *(typename RowVec<T>::type*)&sx[lds_at<kTK>(r, c)] =
-          __builtin_convertvector(v, typename RowVec<T>::type);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s < kTM; s += 16) {
-      short8v fy[2], fx[2];
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        fy[i] = read_fragment<kTN>(sy, s, wn + i * 32);
-        fx[i] = read_fragment<kTK>(sx, s, wk + i * 32);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-          acc[i][j] = mfma<T>(fy[i], fx[j], acc[i][j]);
-    }
-    __syncthreads();
+    cur = nxt;
   }
 
   // element i of a lane: row 8 * (i / 4) + 4 * (lane / 32) + i % 4 of the
   // 32 by 32 block, column lane % 32
 #pragma unroll
-  for (int bi = 0; bi < 2; bi++)
+  for (int bi = 0; bi < FN; bi++)
 #pragma unroll
-    for (int bj = 0; bj < 2; bj++)
+    for (int i = 0; i < 16; i++) {
+      const int64_t n =
+          n0 + wn + bi * 32 + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
+      if (n >= p.n) continue;
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const int64_t n = n0 + wn + bi * 32 + 8 * (i / 4) + 4 * (lane / 32) +
-                          i % 4;
+      for (int bj = 0; bj < FK; bj++) {
         const int64_t k = k0 + wk + bj * 32 + lane % 32;
-        if (n >= a.n || k >= a.k) continue;
+        if (k >= p.k) continue;
         if (p.slices > 1)
-          p.partial[(blockIdx.z * a.n + n) * a.k + k] = acc[bi][bj][i];
+          p.partial[(blockIdx.y * p.n + n) * p.k + k] = acc[bi][bj][i];
         else
-          ((O*)a.dw)[n * a.k + k] = (O)acc[bi][bj][i];
+          ((O*)p.dw)[n * p.k + k] = (O)acc[bi][bj][i];
       }
+    }
 }
 
 // dW from the slices' sums, in their order.
@@ -180,29 +307,41 @@ __global__ __launch_bounds__(kThreads) void wgrad_join_kernel(
   }
 }
 
-// An fp32 gradient as three bf16 planes of 8 bits of its significand each,
-// cut off rather than rounded so that no plane can pass the largest number:
-// their sum is the value itself, up to the last bits of numbers near the
-// smallest.  A NaN or an infinity is whole in the first plane.
-__global__ __launch_bounds__(kThreads) void split_kernel(
-    const float* dy, int64_t dstride, int64_t m, int64_t n, bf16* planes,
+// Gradients that the product cannot read as they are, laid out anew: rows
+// `pitch` elements apart (a multiple of 8), zeros in the columns and, for each
+// plane, the rows that fill the last tile.
+//
+// An fp32 gradient becomes three bf16 planes of 8 bits of its significand
+// each, cut off rather than rounded so that no plane can pass the largest
+// number: their sum is the value itself, up to the last bits of numbers near
+// the smallest.  A NaN or an infinity is whole in the first plane.
+template <typename T, typename P>
+__global__ __launch_bounds__(kThreads) void layout_kernel(
+    const T* dy, int64_t dstride, int64_t m, int64_t n, P* out, int64_t rows,
     int64_t pitch) {
-  const int64_t cols = (n + kVec - 1) / kVec;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < m * cols;
-       i += (int64_t)gridDim.x * kThreads) {
+  constexpr int kPlanes = std::is_same_v<T, float> ? 3 : 1;
+  const int64_t cols = pitch / kVec;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+       i < rows * cols; i += (int64_t)gridDim.x * kThreads) {
     const int64_t r = i / cols, c = i % cols * kVec;
-    float8 v = load_upto(dy + r * dstride + c, (int)(n - c < kVec ? n - c : kVec));
+    float8 v = 0.f;
+    if (r < m && c < n)
+      v = load_upto(dy + r * dstride + c, (int)(n - c < kVec ? n - c : kVec));
+    if constexpr (kPlanes == 1) {
+      store8(out + r * pitch + c, v);
+    } else {
 #pragma unroll
-    for (int p = 0; p < 3; p++) {
-      float8 h;
+      for (int p = 0; p < kPlanes; p++) {
+        float8 h;
 #pragma unroll
-      for (int j = 0; j < kVec; j++) {
-        h[j] = is_finite(v[j])
-                   ? __uint_as_float(__float_as_uint(v[j]) & 0xffff0000u)
-                   : v[j];
-        v[j] = is_finite(v[j]) ? v[j] - h[j] : 0.f;
+        for (int j = 0; j < kVec; j++) {
+          h[j] = is_finite(v[j])
+                     ? __uint_as_float(__float_as_uint(v[j]) & 0xffff0000u)
+                     : v[j];
+          v[j] = is_finite(v[j]) ? v[j] - h[j] : 0.f;
+        }
+        store8(out + (p * rows + r) * pitch + c, h);
       }
-      store8(planes + (p * m + r) * pitch + c, h);
     }
   }
 }
@@ -244,9 +383,10 @@ __global__ __launch_bounds__(kThreads) void column_join_kernel(
 }
 
 struct Plan {
-  int planes, slices;
-  int64_t slice_rows, pitch, strip_rows, strips;
-  size_t plane_bytes, partial_bytes, strip_bytes;
+  bool big, laid_out;
+  int planes, slices, slice_tiles, xtiles, ntiles, ktiles;
+  int64_t pitch, strip_rows, strips;
+  size_t laid_bytes, partial_bytes, strip_bytes;
 };
 
 size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
@@ -254,18 +394,30 @@ size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
 Plan plan_of(const Act8Wgrad& a) {
   Plan p = {};
   p.planes = a.type == ElemType::kF32 ? 3 : 1;
-  p.pitch = (a.n + 7) / 8 * 8;
-  if (p.planes > 1)
-    p.plane_bytes = round256((size_t)3 * a.m * p.pitch * sizeof(bf16));
-  // Few tiles leave compute units idle: the rows are then cut in slices.
-  const int64_t tiles =
-      ((a.n + kTN - 1) / kTN) * ((a.k + kTK - 1) / kTK);
-  const int64_t rows = p.planes * a.m;
-  int64_t slices = 512 / tiles, most = rows / 256;
-  if (slices > most) slices = most;
+  // The product reads rows of dy in aligned 16-byte pieces.
+  p.laid_out = p.planes > 1 || a.n % 8 || a.dstride % 8 ||
+               a.dstride < a.n || a.dstride > kAct8MaxCols || ((uintptr_t)a.dy & 15);
+  p.pitch = p.laid_out ? (a.n + 7) / 8 * 8 : a.dstride;
+  p.xtiles = (int)((a.m + kTM - 1) / kTM);
+  if (p.laid_out)
+    p.laid_bytes =
+        round256((size_t)p.planes * p.xtiles * kTM * p.pitch * 2);
+  // Tiles of 256 by 256 need half of the LDS reads that tiles of 128 by 128
+  // do for the same work, but leave more of a small dW's edge empty and cut
+  // it in fewer pieces.
+  p.big = a.n > 512 && a.k > 512;
+  const int size = p.big ? 256 : 128;
+  p.ntiles = (int)((a.n + size - 1) / size);
+  p.ktiles = (int)((a.k + size - 1) / size);
+  // Few tiles leave compute units idle: the rows are then cut in slices of
+  // at least four tiles.
+  const int64_t tiles = (int64_t)p.planes * p.xtiles;
+  const int64_t places = p.big ? 256 : 512;
+  int64_t slices = places / ((int64_t)p.ntiles * p.ktiles);
+  if (slices > tiles / 4) slices = tiles / 4;
   if (slices < 1) slices = 1;
-  p.slice_rows = ((rows + slices - 1) / slices + kTM - 1) / kTM * kTM;
-  p.slices = (int)((rows + p.slice_rows - 1) / p.slice_rows);
+  p.slice_tiles = (int)((tiles + slices - 1) / slices);
+  p.slices = (int)((tiles + p.slice_tiles - 1) / p.slice_tiles);
   if (p.slices > 1)
     p.partial_bytes = round256((size_t)p.slices * a.n * a.k * sizeof(float));
   if (a.db) {
@@ -276,56 +428,82 @@ Plan plan_of(const Act8Wgrad& a) {
   return p;
 }
 
+template <typename T, typename O>
+void launch_product(const Plan& plan, const Product& p, hipStream_t stream) {
+  const dim3 grid((uint32_t)(plan.ntiles * plan.ktiles),
+                  (uint32_t)plan.slices);
+  if (plan.big)
+    launch(act8_wgrad_kernel<T, O, 4, 4>, grid, kThreads, stream, p);
+  else
+    launch(act8_wgrad_kernel<T, O, 2, 2>, grid, kThreads, stream, p);
+}
+
+uint32_t flat_grid(int64_t items) {
+  const int64_t want = (items + kThreads - 1) / kThreads;
+  return (uint32_t)(want < 4096 ? want : 4096);
+}
+
 }  // namespace
 
 size_t act8_wgrad_workspace(const Act8Wgrad& a) {
   if (a.m == 0 || a.n == 0 || a.k == 0) return 0;
   const Plan p = plan_of(a);
-  return p.plane_bytes + p.partial_bytes + p.strip_bytes;
+  return p.laid_bytes + p.partial_bytes + p.strip_bytes;
 }
 
 hipError_t act8_wgrad(const Act8Wgrad& a, hipStream_t stream) {
   if (a.m == 0 || a.n == 0 || a.k == 0) return hipSuccess;
+  if (a.n > kAct8MaxCols || a.pitch > kAct8MaxCols) return hipErrorInvalidValue;
   const Plan plan = plan_of(a);
-  char* ws = (char*)a.workspace;
-  float* strips = (float*)(ws + plan.plane_bytes + plan.partial_bytes);
-  Product p = {a.dy,        a.dstride,        0,
-               plan.planes, plan.slices,      plan.slice_rows,
-               (float*)(ws + plan.plane_bytes)};
-  const dim3 grid((uint32_t)((a.n + kTN - 1) / kTN),
-                  (uint32_t)((a.k + kTK - 1) / kTK), (uint32_t)plan.slices);
-  if (grid.y > 65535 || (int64_t)grid.x * grid.y * grid.z >= (1 << 24))
+  if ((int64_t)plan.ntiles * plan.ktiles * plan.slices > (1 << 23) ||
+      plan.slices > 65535)
     return hipErrorInvalidValue;
-  if (a.type == ElemType::kF32) {
-    bf16* planes = (bf16*)ws;
-    const int64_t items = a.m * ((a.n + 7) / 8);
-    const int64_t want = (items + kThreads - 1) / kThreads;
-    launch(split_kernel, (uint32_t)(want < 4096 ? want : 4096), kThreads, stream, (const float*)a.dy, a.dstride, a.m, a.n, planes,
-                             plan.pitch);
-    p.dy = planes;
-    p.dstride = plan.pitch;
-    p.plane = a.m * plan.pitch;
-    launch(act8_wgrad_kernel<bf16, float>, grid, kThreads, stream, a, p);
-  } else if (a.type == ElemType::kBF16) {
-    launch(act8_wgrad_kernel<bf16, bf16>, grid, kThreads, stream, a, p);
-  } else {
-    launch(act8_wgrad_kernel<fp16, fp16>, grid, kThreads, stream, a, p);
-  }
+  char* ws = (char*)a.workspace;
+  float* strips = (float*)(ws + plan.laid_bytes + plan.partial_bytes);
+  const int64_t laid_rows = (int64_t)plan.xtiles * kTM;
+  Product p = {};
+  p.dpitch = (int)(plan.pitch * 2);
+  p.cpitch = (int)a.pitch;
+  p.dy.base = plan.laid_out ? ws : (const char*)a.dy;
+  p.dy.bytes = plan.laid_out
+                   ? plan.planes * laid_rows * plan.pitch * 2
+                   : ((a.m - 1) * a.dstride + a.n) * 2;
+  p.dy.tile = (int64_t)kTM * plan.pitch * 2;
+  p.codes = {(const char*)a.codes, a.m * a.pitch, kTM * a.pitch};
+  p.exps = {(const char*)a.exps, a.m * a.pitch / kAct8Group,
+            kTM * a.pitch / kAct8Group};
+  p.xtiles = plan.xtiles;
+  p.tiles = plan.planes * plan.xtiles;
+  p.slices = plan.slices;
+  p.slice_tiles = plan.slice_tiles;
+  p.ntiles = plan.ntiles;
+  p.ktiles = plan.ktiles;
+  p.n = a.n;
+  p.k = a.k;
+  p.dw = a.dw;
+  p.partial = (float*)(ws + plan.laid_bytes);
   with_type(a.type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
+    using P = std::conditional_t<std::is_same_v<T, float>, bf16, T>;
+    if (plan.laid_out)
+      launch(layout_kernel<T, P>, flat_grid(laid_rows * plan.pitch / kVec),
+             kThreads, stream, (const T*)a.dy, a.dstride, a.m, a.n, (P*)ws,
+             laid_rows, plan.pitch);
+    launch_product<P, T>(plan, p, stream);
     if (plan.slices > 1) {
       const int64_t count = a.n * a.k;
-      const int64_t want = (count + kThreads * kVec - 1) / (kThreads * kVec);
-      launch(wgrad_join_kernel<T>, (uint32_t)(want < 4096 ? want : 4096), kThreads, stream, 
-              p.partial, plan.slices, count, (T*)a.dw);
+      launch(wgrad_join_kernel<T>, flat_grid((count + kVec - 1) / kVec),
+             kThreads, stream, (const float*)p.partial, plan.slices, count,
+             (T*)a.dw);
     }
     if (a.db) {
       const dim3 sums((uint32_t)((a.n + kSumCols - 1) / kSumCols),
                       (uint32_t)plan.strips);
-      launch(column_strip_kernel<T>, sums, kSumCols * kSumLanes, stream, 
-          (const T*)a.dy, a.dstride, a.m, a.n, plan.strip_rows,
-          strips);
-      launch(column_join_kernel<T>, (uint32_t)((a.n + kThreads - 1) / kThreads), kThreads, stream, strips, (int)plan.strips, a.n, (T*)a.db);
+      launch(column_strip_kernel<T>, sums, kSumCols * kSumLanes, stream,
+             (const T*)a.dy, a.dstride, a.m, a.n, plan.strip_rows, strips);
+      launch(column_join_kernel<T>,
+             (uint32_t)((a.n + kThreads - 1) / kThreads), kThreads, stream,
+             (const float*)strips, (int)plan.strips, a.n, (T*)a.db);
     }
   });
   return hipGetLastError();

@@ -78,25 +78,77 @@ __device__ inline float8 widen(V v) {
   return __builtin_convertvector(v, float8);
 }
 
-// A vector of weights held in fp32 or in T.
-template <typename T>
-__device__ inline float8 weight_upto(const void* p, bool f32, int64_t i,
-                                     int n) {
-  return f32 ? load_upto((const float*)p + i, n) : load_upto((const T*)p + i, n);
-}
-
-template <typename T>
-__device__ inline void put_weight_upto(void* p, bool f32, int64_t i, float8 v,
-                                       int n) {
-  if (f32)
-    store_upto((float*)p + i, v, n);
-  else
-    store_upto((T*)p + i, v, n);
-}
-
 __device__ inline float sum8(float8 v) {
   return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
 }
+
+// The columns of a row that one lane takes: 8 from `col` on.  The lane at the
+// row's end moves back so that its 8 lie inside the row, and shares `dup`
+// columns with the lane before it: both compute the same there and write the
+// same, and only sums over the row leave the shared ones out.  So no access
+// needs a count, which would cost registers and branches at each.  A lane
+// with dup == 8 has nothing of its own.  kTiny: rows of fewer than 8 columns,
+// which one lane takes element by element.
+template <bool kTiny>
+struct Cols {
+  int col, dup, count;
+  __device__ inline Cols() {}
+  __device__ inline Cols(int at, int dim) {
+    count = kTiny ? dim : kVec;
+    col = kTiny ? 0 : at + kVec <= dim ? at : dim - kVec;
+    dup = kTiny ? (at ? kVec : 0) : at >= dim ? kVec : at - col;
+  }
+  __device__ inline bool own() const { return dup < kVec; }
+  template <typename T>
+  __device__ inline typename RowVec<T>::type raw(const T* row) const {
+    if constexpr (kTiny) return raw_upto(row, count);
+    return *(const typename RowVec<T>::unaligned*)(row + col);
+  }
+  template <typename T>
+  __device__ inline float8 load(const T* row) const {
+    return widen(raw(row));
+  }
+  // A vector of weights held in fp32 or in T, `at` elements into p.
+  template <typename T>
+  __device__ inline float8 weight(const void* p, bool f32, int64_t at) const {
+    return f32 ? load((const float*)p + at) : load((const T*)p + at);
+  }
+  template <typename T>
+  __device__ inline void store(T* row, float8 v) const {
+    if constexpr (kTiny)
+      store_upto(row, v, count);
+    else
+      store8(row + col, v);
+  }
+  template <typename T>
+  __device__ inline void put_weight(void* p, bool f32, int64_t at,
+                                    float8 v) const {
+    if (f32)
+      store((float*)p + at, v);
+    else
+      store((T*)p + at, v);
+  }
+  // row += v, or row = v, on the lane's own columns.
+  __device__ inline void accumulate(float* row, float8 v, bool first) const {
+    if (!kTiny && dup == 0) {
+      if (!first) v += load8(row + col);
+      store8(row + col, v);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; i++)
+      if (i >= dup && i < count) row[col + i] = first ? v[i] : row[col + i] + v[i];
+  }
+  // The sum of the lane's own columns.
+  __device__ inline float sum(float8 v) const {
+    if (dup) {
+#pragma unroll
+      for (int i = 0; i < kVec; i++) v[i] = i < dup ? 0.f : v[i];
+    }
+    return sum8(v);
+  }
+};
+
 
 // Launches a kernel without dynamic LDS.
 template <typename... P>

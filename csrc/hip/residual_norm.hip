@@ -59,39 +59,40 @@ constexpr int block_of() {
   return TPR < 256 ? 256 : TPR;
 }
 
-template <typename T, int TPR, int VPT>
+// The team of a thread: its wave where that is a team, as a uniform number.
+template <int TPR>
+__device__ inline int team_of() {
+  if constexpr (TPR >= 256) return 0;
+  return __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+}
+
+template <typename T, int TPR, int VPT, bool kTiny>
 __global__ __launch_bounds__(block_of<TPR>()) void norm_forward_kernel(
     NormFwd a) {
   constexpr int kTeams = block_of<TPR>() / TPR;
   __shared__ float red[2][TPR / kWave];
-  const int lane = threadIdx.x % TPR, team = threadIdx.x / TPR;
+  const int lane = threadIdx.x % TPR, team = team_of<TPR>();
   const int64_t step = (int64_t)gridDim.x * kTeams;
   const float inv_dim = 1.f / (float)a.dim;
-  int64_t col[VPT];
-  int m[VPT];
+  Cols<kTiny> c[VPT];
   float8 coef[VPT], pre[VPT];  // bs * post, and the group's gate if it is one
   const bool fixed_gate = a.gmode == Gate::kGroup && a.group_rows >= a.rows;
 #pragma unroll
   for (int j = 0; j < VPT; j++) {
-    col[j] = ((int64_t)j * TPR + lane) * kVec;
-    const int64_t left = a.dim - col[j];
-    m[j] = left < 0 ? 0 : left < kVec ? (int)left : kVec;
-    if (m[j] == 0) col[j] = 0;
+    c[j] = Cols<kTiny>((j * TPR + lane) * kVec, (int)a.dim);
     coef[j] = a.branch_scale;
     pre[j] = 1.f;
-    if (a.post) coef[j] *= weight_upto<T>(a.post, a.post32, col[j], m[j]);
-    if (a.pre) pre[j] = weight_upto<T>(a.pre, a.pre32, col[j], m[j]);
-    if (fixed_gate)
-      coef[j] *= weight_upto<T>(a.gate, a.gate32, col[j], m[j]);
+    if (a.post) coef[j] *= c[j].template weight<T>(a.post, a.post32, 0);
+    if (a.pre) pre[j] = c[j].template weight<T>(a.pre, a.pre32, 0);
+    if (fixed_gate) coef[j] *= c[j].template weight<T>(a.gate, a.gate32, 0);
   }
   typename RowVec<T>::type xn[VPT], on[VPT];
   int64_t row = (int64_t)blockIdx.x * kTeams + team;
   auto fetch = [&](int64_t r) {
 #pragma unroll
     for (int j = 0; j < VPT; j++) {
-      xn[j] = raw_upto((const T*)a.x + r * a.xstride + col[j], m[j]);
-      if (a.branch)
-        on[j] = raw_upto((const T*)a.branch + r * a.bstride + col[j], m[j]);
+      xn[j] = c[j].raw((const T*)a.x + r * a.xstride);
+      if (a.branch) on[j] = c[j].raw((const T*)a.branch + r * a.bstride);
     }
   };
   if (row < a.rows) fetch(row);
@@ -108,7 +109,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_forward_kernel(
       if (a.post) {
         float s[1] = {0.f};
 #pragma unroll
-        for (int j = 0; j < VPT; j++) s[0] += sum8(o[j] * o[j]);
+        for (int j = 0; j < VPT; j++) s[0] += c[j].sum(o[j] * o[j]);
         row_sums<TPR>(s, red[0]);
         ro = 1.f / sqrtf(s[0] * inv_dim + a.eps);
         if (lane == 0 && a.rbranch) a.rbranch[row] = ro;
@@ -123,23 +124,23 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_forward_kernel(
         at = (int64_t)((uint32_t)row / (uint32_t)a.group_rows) * a.dim;
 #pragma unroll
       for (int j = 0; j < VPT; j++) {
-        float8 c = coef[j] * g;
-        if (at >= 0) c *= weight_upto<T>(a.gate, a.gate32, at + col[j], m[j]);
-        y[j] += c * o[j];
-        if (m[j]) store_upto((T*)a.y + row * a.dim + col[j], y[j], m[j]);
+        float8 k = coef[j] * g;
+        if (at >= 0) k *= c[j].template weight<T>(a.gate, a.gate32, at);
+        y[j] += k * o[j];
+        if (c[j].own()) c[j].store((T*)a.y + row * a.dim, y[j]);
       }
     }
     if (a.h) {
       float s[1] = {0.f};
 #pragma unroll
-      for (int j = 0; j < VPT; j++) s[0] += sum8(y[j] * y[j]);
+      for (int j = 0; j < VPT; j++) s[0] += c[j].sum(y[j] * y[j]);
       row_sums<TPR>(s, red[1]);
       const float ry = 1.f / sqrtf(s[0] * inv_dim + a.eps);
       if (lane == 0 && a.ry) a.ry[row] = ry;
 #pragma unroll
       for (int j = 0; j < VPT; j++)
-        if (m[j])
-          store_upto((T*)a.h + row * a.dim + col[j], y[j] * ry * pre[j], m[j]);
+        if (c[j].own())
+          c[j].store((T*)a.h + row * a.dim, y[j] * ry * pre[j]);
     }
   }
 }
@@ -157,7 +158,11 @@ struct Parts {
   float *pre, *post, *group;
 };
 
-template <typename T, int TPR, int VPT>
+// kSeam: the whole seam (branch with its norm, both gradients, a gate of
+// groups or none), as every block of a network but the first has it.  Left to
+// the arguments, these choices cost about 60 registers and with them half of
+// the waves in flight.
+template <typename T, int TPR, int VPT, bool kTiny, bool kSeam>
 __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
     NormBwd a, Cut cut, Parts parts) {
   constexpr int kTeams = block_of<TPR>() / TPR;
@@ -165,24 +170,55 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
   // the teams' column sums on their way to the first team
   __shared__ float joint[kTeams > 1 ? kTeams - 1 : 1]
                         [kTeams > 1 ? TPR * VPT * kVec : 1];
-  const int lane = threadIdx.x % TPR, team = threadIdx.x / TPR;
-  const float inv_dim = 1.f / (float)a.dim;
-  const bool grouped = a.gmode == Gate::kGroup;
+  // wide rows: sums over rows that registers have no room for, for each lane
+  constexpr bool kWide = TPR * VPT > 1024;
+  __shared__ float held[kWide ? 2 * TPR * VPT * kVec : 1];
+  const bool has_branch = kSeam || a.branch, has_post = kSeam || a.post;
+  const bool has_dy = kSeam || a.dy, has_dh = kSeam || a.dh;
+  const Gate gmode = kSeam && a.gmode != Gate::kNone ? Gate::kGroup : a.gmode;
+  const bool full = !kSeam && gmode == Gate::kFull;
+  const bool per_row = !kSeam && gmode == Gate::kRow;
+  const bool grouped = gmode == Gate::kGroup;
   const bool one_gate = grouped && cut.groups == 1;
-  int64_t col[VPT];
-  int m[VPT];
-  float8 post[VPT], pre[VPT], gate[VPT];
-  float8 acc_pre[VPT], acc_post[VPT], acc_all[VPT];
+  const int lane = threadIdx.x % TPR, team = team_of<TPR>();
+  const float inv_dim = 1.f / (float)a.dim;
+  Cols<kTiny> c[VPT];
+  // pre, and bs * post * gate (without the gate of a row or an element);
+  // wide rows read them again at each use
+  float8 pre[VPT], coef[VPT], acc_pre[VPT], acc_post[VPT];
+  auto held_at = [&](int what, int j) -> float8& {
+    return *(float8*)&held[((what * VPT + j) * TPR + lane) * kVec];
+  };
+  auto add_pre = [&](int j, float8 v) {
+    if constexpr (kWide)
+      held_at(0, j) += v;
+    else
+      acc_pre[j] += v;
+  };
+  auto add_post = [&](int j, float8 v) {
+    if constexpr (kWide)
+      held_at(1, j) += v;
+    else
+      acc_post[j] += v;
+  };
+  auto post_at = [&](int j) {
+    return has_post ? c[j].template weight<T>(a.post, a.post32, 0)
+                    : (float8)1.f;
+  };
+  auto pre_at = [&](int j) {
+    return a.pre ? c[j].template weight<T>(a.pre, a.pre32, 0) : (float8)1.f;
+  };
+  auto gate_at = [&](int j, int64_t at) {
+    return c[j].template weight<T>(a.gate, a.gate32, at);
+  };
 #pragma unroll
   for (int j = 0; j < VPT; j++) {
-    col[j] = ((int64_t)j * TPR + lane) * kVec;
-    const int64_t left = a.dim - col[j];
-    m[j] = left < 0 ? 0 : left < kVec ? (int)left : kVec;
-    if (m[j] == 0) col[j] = 0;
-    post[j] = pre[j] = gate[j] = 1.f;
-    if (a.post) post[j] = weight_upto<T>(a.post, a.post32, col[j], m[j]);
-    if (a.pre) pre[j] = weight_upto<T>(a.pre, a.pre32, col[j], m[j]);
-    acc_pre[j] = acc_post[j] = acc_all[j] = 0.f;
+    c[j] = Cols<kTiny>((j * TPR + lane) * kVec, (int)a.dim);
+    if constexpr (!kWide) pre[j] = pre_at(j);
+    if constexpr (kWide)
+      held_at(0, j) = held_at(1, j) = 0.f;
+    else
+      acc_pre[j] = acc_post[j] = 0.f;
   }
   // Adds the teams' sums up in the first team, in the order of the teams.
   auto join = [&](float8 (&v)[VPT]) {
@@ -203,12 +239,11 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
       }
     }
   };
-  auto put = [&](float* part, int64_t at, const float8 (&v)[VPT]) {
-    if (team == 0) {
+
+  auto take = [&](int what, float8 (&v)[VPT]) {
 #pragma unroll
-      for (int j = 0; j < VPT; j++)
-        if (m[j]) store_upto(part + at * a.dim + col[j], v[j], m[j]);
-    }
+    for (int j = 0; j < VPT; j++)
+      if constexpr (kWide) v[j] = held_at(what, j);
   };
 
   const int64_t slice = blockIdx.x % cut.slices;
@@ -221,129 +256,150 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
     int64_t last = first + cut.slice_rows;
     if (last > (grp + 1) * cut.group_rows) last = (grp + 1) * cut.group_rows;
     if (last > a.rows) last = a.rows;
-    if (grouped) {
+    auto coef_at = [&](int j) {
+      float8 v = post_at(j) * a.branch_scale;
+      if (grouped) v *= gate_at(j, grp * a.dim);
+      return v;
+    };
+    if constexpr (!kWide) {
 #pragma unroll
-      for (int j = 0; j < VPT; j++)
-        gate[j] = weight_upto<T>(a.gate, a.gate32, grp * a.dim + col[j], m[j]);
+      for (int j = 0; j < VPT; j++) coef[j] = coef_at(j);
     }
     typename RowVec<T>::type xn[VPT], on[VPT], dyn[VPT], dhn[VPT];
     float ro_n = 1.f, ry_n = 0.f, g_n = 1.f;
     auto fetch = [&](int64_t r) {
 #pragma unroll
       for (int j = 0; j < VPT; j++) {
-        if (a.dh) {
-          xn[j] = raw_upto((const T*)a.x + r * a.xstride + col[j], m[j]);
-          dhn[j] = raw_upto((const T*)a.dh + r * a.dhstride + col[j], m[j]);
+        if (has_dh) {
+          xn[j] = c[j].raw((const T*)a.x + r * a.xstride);
+          dhn[j] = c[j].raw((const T*)a.dh + r * a.dhstride);
         }
-        if (a.dy)
-          dyn[j] = raw_upto((const T*)a.dy + r * a.dystride + col[j], m[j]);
-        if (a.branch)
-          on[j] = raw_upto((const T*)a.branch + r * a.bstride + col[j], m[j]);
+        if (has_dy)
+          dyn[j] = c[j].raw((const T*)a.dy + r * a.dystride);
+        if (has_branch)
+          on[j] = c[j].raw((const T*)a.branch + r * a.bstride);
       }
-      if (a.dh) ry_n = a.ry[r];
-      if (a.branch && a.post) ro_n = a.rbranch[r];
-      if (a.gmode == Gate::kRow)
+      if (has_dh) ry_n = a.ry[r];
+      if (has_branch && has_post) ro_n = a.rbranch[r];
+      if (per_row)
         g_n = a.gate32 ? ((const float*)a.gate)[r]
                        : (float)((const T*)a.gate)[r];
     };
     int64_t row = first + team;
-    if (row < last) fetch(row);
+    if (!kWide && row < last) fetch(row);
     for (; row < last; row += kTeams) {
+      if (kWide) fetch(row);
       const float ry = ry_n, ro = ro_n, g_row = g_n;
-      float8 dY[VPT], no[VPT], ny[VPT], g[VPT];
-      // sums: ny * t;  q * (dy + ry * t);  q * ny, with q = no * post * gate:
-      // the mean that do needs then follows without a second pass.
+      float8 dY[VPT], no[VPT], ny[VPT];
+      // sums: ny * t;  q * (dy + ry * t);  q * ny, with q = coef * no (and an
+      // element's gate): the mean that do needs then follows without a second
+      // pass over the row.
       float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < VPT; j++) {
         ny[j] = dY[j] = 0.f;
-        float8 c;
-        if (a.branch) {
+        float8 q;
+        if (has_branch) {
           no[j] = widen(on[j]) * ro;
-          g[j] = gate[j] * g_row;
-          if (a.gmode == Gate::kFull)
-            g[j] = weight_upto<T>(a.gate, a.gate32, row * a.dim + col[j], m[j]);
-          c = no[j] * post[j];
+          q = no[j] * (kWide ? coef_at(j) : coef[j]);
+          if (full) q *= gate_at(j, row * a.dim);
         }
-        if (a.dy) dY[j] = widen(dyn[j]);
-        if (a.dh) {
+        if (has_dy) dY[j] = widen(dyn[j]);
+        if (has_dh) {
           const float8 dh = widen(dhn[j]);
           float8 y = widen(xn[j]) * a.residual_scale;
-          if (a.branch) y += c * g[j] * a.branch_scale;
+          if (has_branch) y += q * g_row;
           ny[j] = y * ry;
-          const float8 t = dh * pre[j];
-          acc_pre[j] += dh * ny[j];
+          const float8 t = dh * (kWide ? pre_at(j) : pre[j]);
+          add_pre(j, dh * ny[j]);
           dY[j] += t * ry;
-          s[0] += sum8(ny[j] * t);
+          s[0] += c[j].sum(ny[j] * t);
         }
-        if (a.branch) {
-          const float8 q = c * (a.gmode == Gate::kFull ? g[j] : gate[j]);
-          s[1] += sum8(q * dY[j]);
-          s[2] += sum8(q * ny[j]);
+        if (has_branch) {
+          s[1] += c[j].sum(q * dY[j]);
+          s[2] += c[j].sum(q * ny[j]);
         }
       }
-      if (row + kTeams < last) fetch(row + kTeams);
+      if (!kWide && row + kTeams < last) fetch(row + kTeams);
       row_sums<TPR>(s, red[parity]);
       parity ^= 1;
       const float k0 = ry * s[0] * inv_dim;
-      // sum of no * post * gate * dY, without the row's own gate
+      // sum of q * dY, without the row's own gate
       const float sq = s[1] - k0 * s[2];
-      const float k1 = sq * a.branch_scale * g_row * inv_dim;
-      if (a.gmode == Gate::kRow && a.dgate && lane == 0) {
-        const float dg = sq * a.branch_scale;
+      const float k1 = sq * g_row * inv_dim;
+      if (per_row && a.dgate && lane == 0) {
         if (a.gate32)
-          ((float*)a.dgate)[row] = dg;
+          ((float*)a.dgate)[row] = sq;
         else
-          ((T*)a.dgate)[row] = (T)dg;
+          ((T*)a.dgate)[row] = (T)sq;
       }
 #pragma unroll
       for (int j = 0; j < VPT; j++) {
         dY[j] -= ny[j] * k0;
-        if (m[j])
-          store_upto((T*)a.dx + row * a.dim + col[j],
-                     dY[j] * a.residual_scale, m[j]);
-        if (a.branch) {
-          const float8 du = dY[j] * g[j] * a.branch_scale;
-          float8 db = du * post[j];
-          if (a.post) db = (db - no[j] * k1) * ro;
-          if (m[j])
-            store_upto((T*)a.dbranch + row * a.dim + col[j], db, m[j]);
-          if (a.gmode == Gate::kFull && a.dgate && m[j])
-            put_weight_upto<T>(a.dgate, a.gate32, row * a.dim + col[j],
-                               dY[j] * no[j] * post[j] * a.branch_scale, m[j]);
-          const float8 e = dY[j] * no[j];
-          acc_post[j] += grouped ? e : e * g[j];
+        if (c[j].own())
+          c[j].store((T*)a.dx + row * a.dim, dY[j] * a.residual_scale);
+        if (has_branch) {
+          float8 e = dY[j] * no[j];
+          const float8 k = kWide ? coef_at(j) : coef[j];
+          float8 du = dY[j] * k * g_row;
+          if (full) {
+            const float8 g = gate_at(j, row * a.dim);
+            if (a.dgate && c[j].own())
+              c[j].template put_weight<T>(a.dgate, a.gate32, row * a.dim,
+                                          e * k);
+            e *= g;
+            du *= g;
+          }
+          add_post(j, e * g_row);
+          if (has_post) du = (du - no[j] * k1) * ro;
+          if (c[j].own()) c[j].store((T*)a.dbranch + row * a.dim, du);
         }
       }
     }
     if (grouped && !one_gate) {
-      // the group's sum goes out, and on into dpost's
+      take(1, acc_post);
+      // the group's sum of dY * no goes out, and on into dpost's
       join(acc_post);
       if (team == 0) {
 #pragma unroll
         for (int j = 0; j < VPT; j++) {
-          if (a.dgate && cut.slices == 1 && m[j])
-            put_weight_upto<T>(a.dgate, a.gate32, grp * a.dim + col[j],
-                               acc_post[j] * post[j] * a.branch_scale, m[j]);
-          acc_all[j] += acc_post[j] * gate[j];
+          if (!c[j].own()) continue;
+          if (a.dgate && cut.slices == 1)
+            c[j].template put_weight<T>(
+                a.dgate, a.gate32, grp * a.dim,
+                acc_post[j] * post_at(j) * a.branch_scale);
+          if (parts.group)
+            c[j].store(parts.group + blockIdx.x * a.dim, acc_post[j]);
+          if (parts.post)
+            c[j].accumulate(parts.post + blockIdx.x * a.dim,
+                            acc_post[j] * gate_at(j, grp * a.dim), grp == g0);
         }
       }
-      if (a.dgate && cut.slices > 1) put(parts.group, blockIdx.x, acc_post);
 #pragma unroll
-      for (int j = 0; j < VPT; j++) acc_post[j] = 0.f;
+      for (int j = 0; j < VPT; j++) {
+        if constexpr (kWide)
+          held_at(1, j) = 0.f;
+        else
+          acc_post[j] = 0.f;
+      }
     }
   }
+  auto put = [&](float* part, const float8 (&v)[VPT]) {
+    if (team == 0) {
+#pragma unroll
+      for (int j = 0; j < VPT; j++)
+        if (c[j].own()) c[j].store(part + blockIdx.x * a.dim, v[j]);
+    }
+  };
   if (parts.pre) {
+    take(0, acc_pre);
     join(acc_pre);
-    put(parts.pre, blockIdx.x, acc_pre);
+    put(parts.pre, acc_pre);
   }
-  if (parts.post) {
-    if (grouped && !one_gate) {
-      put(parts.post, blockIdx.x, acc_all);
-    } else {
-      join(acc_post);
-      put(parts.post, blockIdx.x, acc_post);
-    }
+  if (parts.post && !(grouped && !one_gate)) {
+    take(1, acc_post);
+    join(acc_post);
+    put(parts.post, acc_post);
   }
 }
 
@@ -438,20 +494,27 @@ bool wants_group(const NormBwd& a, const Cut& c) {
 // Calls f with the team size and vectors per lane that hold `dim` columns.
 template <typename F>
 void with_team(int64_t dim, F&& f) {
-  if (dim <= 512)
-    f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+  if (dim < kVec)
+    f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>(),
+      std::true_type());
+  else if (dim <= 512)
+    f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>(),
+      std::false_type());
   else if (dim <= 1024)
-    f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+    f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>(),
+      std::false_type());
   else if (dim <= 2048)
-    f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
+    f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>(),
+      std::false_type());
   else if (dim <= 4096)
-    f(std::integral_constant<int, 512>(), std::integral_constant<int, 1>());
+    f(std::integral_constant<int, 512>(), std::integral_constant<int, 1>(),
+      std::false_type());
   else if (dim <= 8192)
-    f(std::integral_constant<int, 1024>(), std::integral_constant<int, 1>());
-  else if (dim <= 16384)
-    f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
+    f(std::integral_constant<int, 512>(), std::integral_constant<int, 2>(),
+      std::false_type());
   else
-    f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+    f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>(),
+      std::false_type());
 }
 
 }  // namespace
@@ -461,13 +524,14 @@ hipError_t norm_forward(const NormFwd& a, hipStream_t stream) {
   if (a.dim > kNormMaxDim) return hipErrorInvalidValue;
   with_type(a.type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    with_team(a.dim, [&](auto tpr, auto vpt) {
+    with_team(a.dim, [&](auto tpr, auto vpt, auto tiny) {
       constexpr int kTpr = decltype(tpr)::value, kVpt = decltype(vpt)::value;
+      constexpr bool kTiny = decltype(tiny)::value;
       constexpr int kBlk = block_of<kTpr>();
       const int64_t teams = kBlk / kTpr;
       const int64_t want = (a.rows + teams - 1) / teams;
       const int64_t most = 256 * 2048 / kBlk;
-      launch(norm_forward_kernel<T, kTpr, kVpt>, (uint32_t)(want < most ? want : most), kBlk, stream, a);
+      launch(norm_forward_kernel<T, kTpr, kVpt, kTiny>, (uint32_t)(want < most ? want : most), kBlk, stream, a);
     });
   });
   return hipGetLastError();
@@ -493,9 +557,17 @@ hipError_t norm_backward(const NormBwd& a, hipStream_t stream) {
   if (wants_group(a, c)) parts.group = ws, ws += part;
   with_type(a.type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    with_team(a.dim, [&](auto tpr, auto vpt) {
+    with_team(a.dim, [&](auto tpr, auto vpt, auto tiny) {
       constexpr int kTpr = decltype(tpr)::value, kVpt = decltype(vpt)::value;
-      launch(norm_backward_kernel<T, kTpr, kVpt>, (uint32_t)c.blocks, block_of<kTpr>(), stream, a, c, parts);
+      constexpr bool kTiny = decltype(tiny)::value;
+      const bool seam = a.branch && a.post && a.dy && a.dh &&
+                        (a.gmode == Gate::kNone || a.gmode == Gate::kGroup);
+      if (seam)
+        launch(norm_backward_kernel<T, kTpr, kVpt, kTiny, true>, (uint32_t)c.blocks,
+               block_of<kTpr>(), stream, a, c, parts);
+      else
+        launch(norm_backward_kernel<T, kTpr, kVpt, kTiny, false>, (uint32_t)c.blocks,
+               block_of<kTpr>(), stream, a, c, parts);
     });
     if (parts.pre || parts.post || parts.group) {
       const dim3 grid((uint32_t)((a.dim + kJoinCols - 1) / kJoinCols),

@@ -45,7 +45,7 @@ hipError_t embedding_backward(const EmbeddingBwd& a, hipStream_t stream);
 enum class Gate : int { kNone = 0, kGroup = 1, kRow = 2, kFull = 3 };
 
 // The columns that the kernels hold in registers, at most.
-constexpr int64_t kNormMaxDim = 32768;
+constexpr int64_t kNormMaxDim = 16384;
 
 struct NormFwd {
   const void* x;       // [rows, dim], rows `xstride` elements apart
@@ -99,6 +99,10 @@ hipError_t norm_backward(const NormBwd& a, hipStream_t stream);
 // own.  Rows of codes are `pitch` bytes apart, a multiple of 32, and the
 // columns past the row's end hold zeros.
 constexpr int kAct8Group = 32;
+
+// Columns of a gradient or of codes that one product takes, at most: 64 rows
+// of them are addressed in 31 bits.
+constexpr int64_t kAct8MaxCols = 1 << 23;
 
 struct Act8Move {
   void* x;             // [rows, cols], rows `xstride` elements apart

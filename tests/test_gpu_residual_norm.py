@@ -3,8 +3,8 @@
 
 Tolerances: outputs are rounded once to their type (half a step: eps / 2 of
 the value, and half of float16's smallest step of 2**-24).  Before that all is
-fp32: a sum of at most 32768 terms goes through fewer than 48 additions on any
-path (8 of a vector, 4 vectors, 6 lane exchanges, 16 waves), and the products
+fp32: a sum of at most 16384 terms goes through fewer than 48 additions on any
+path (8 of a vector, 2 vectors, 6 lane exchanges, 16 waves), and the products
 around it add fewer than 16 roundings, so C = 64 half steps of 2**-24, relative
 to the sum of the magnitudes, bound each number before its last rounding.
 Sums over R rows add R roundings.
@@ -127,8 +127,8 @@ def case(shape, dtype=BF, gate=None, post=True, pre=True, wtype=F32,
 
 
 @pytest.mark.parametrize("dim", [1, 2, 7, 64, 511, 512, 513, 1000, 1024, 1025,
-                                 2048, 2049, 4096, 4100, 8192, 8193, 16384,
-                                 16385, 32768])
+                                 2048, 2049, 4096, 4100, 8192, 8193, 12289,
+                                 16383, 16384])
 def test_widths(dim):
     case((2, 5, dim), gate=(dim,), bs=0.5, seed=dim)
     case((2, 5, dim), dtype=F32, gate=(2, 1, dim), bs=0.5, seed=dim + 1)
@@ -164,6 +164,10 @@ def test_gates(gate, post, pre):
     ((2, 7, 33, 264), (2, 7, 1, 264)),
     ((1500, 264), (1500, 1)),
     ((3, 500, 2100), (3, 1, 2100)),
+    ((3, 40, 9001), (3, 1, 9001)),
+    ((600, 2, 9001), (600, 1, 9001)),
+    ((600, 2, 65), (600, 1, 65)),
+    ((600, 2, 5), (600, 1, 5)),
     ((1, 1, 264), (1, 1, 264)),
     ((1, 264), (1, 1)),
 ])

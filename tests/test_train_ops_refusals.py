@@ -29,7 +29,7 @@ TOK = torch.zeros(3, dtype=torch.int64)
     (lambda: ops.rms_norm(_bf(4, 8), _bf(9)), r"weight must be \[8\]"),
     (lambda: ops.rms_norm(_bf(4, 8), torch.zeros(8, dtype=torch.float16)),
      "float32 or of x's type"),
-    (lambda: ops.rms_norm(_bf(2, 32769)), "at most 32768 columns"),
+    (lambda: ops.rms_norm(_bf(2, 16385)), "at most 16384 columns"),
     (lambda: ops.rms_norm(_bf(4, 8), eps=-1.0), "eps"),
     (lambda: ops.rms_norm(_bf(4, 8)), "x must be on the GPU"),
     (lambda: ops.gated_residual_norm(_bf(4, 8), _bf(4, 9)), "x's shape"),
