@@ -272,25 +272,41 @@ void act8_wgrad_kernel(Product p) {
     cur = nxt;
   }
 
-  // element i of a lane: row 8 * (i / 4) + 4 * (lane / 32) + i % 4 of the
-  // 32 by 32 block, column lane % 32
+  // Out through LDS, 32 rows of a wave at a time, so that a lane writes 8
+  // neighbours of a row: written straight from where the matrix instructions
+  // leave them, a tile of 256 by 256 took about 15 us.  Element i of a lane is
+  // that of row 8 * (i / 4) + 4 * (lane / 32) + i % 4 of a 32 by 32 block, and
+  // of column lane % 32; the pitch puts rows 4 apart on different banks.
+  constexpr int kPitch = FK * 32 + 8;
+  static_assert(4 * 32 * kPitch * 2 <= 2 * kTile, "LDS");
+  __syncthreads();
+  float* out = (float*)lds + wave * 32 * kPitch;
+  const int er = lane / (FK * 4), ec = lane % (FK * 4) * kVec;
+  const int64_t ek = k0 + wk + ec;
+  const int em = p.k - ek < kVec ? (int)(p.k - ek) : kVec;
 #pragma unroll
-  for (int bi = 0; bi < FN; bi++)
+  for (int bi = 0; bi < FN; bi++) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const int64_t n =
-          n0 + wn + bi * 32 + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
-      if (n >= p.n) continue;
+    for (int bj = 0; bj < FK; bj++)
 #pragma unroll
-      for (int bj = 0; bj < FK; bj++) {
-        const int64_t k = k0 + wk + bj * 32 + lane % 32;
-        if (k >= p.k) continue;
-        if (p.slices > 1)
-          p.partial[(blockIdx.y * p.n + n) * p.k + k] = acc[bi][bj][i];
-        else
-          ((O*)p.dw)[n * p.k + k] = (O)acc[bi][bj][i];
-      }
+      for (int i = 0; i < 16; i++)
+        out[(8 * (i / 4) + 4 * (lane / 32) + i % 4) * kPitch + bj * 32 +
+            lane % 32] = acc[bi][bj][i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = er; r < 32; r += 16 / FK) {
+      const int64_t n = n0 + wn + bi * 32 + r;
+      const float8 v = *(const float8*)&out[r * kPitch + ec];
+      if (n >= p.n || em <= 0) continue;
+      if (p.slices > 1)
+        store_upto(p.partial + (blockIdx.y * p.n + n) * p.k + ek, v, em);
+      else
+        store_upto((O*)p.dw + n * p.k + ek, v, em);
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
 }
 
 // dW from the slices' sums, in their order.
