@@ -15,6 +15,8 @@
 // own products.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
+
 #include "act8_codes.h"
 
 namespace baguanet {
@@ -97,11 +99,13 @@ struct Stream {
   int64_t tile;       // from one tile to the next
 };
 
-__device__ inline __amdgpu_buffer_rsrc_t at_tile(const Stream& s, int64_t t) {
-  int64_t left = s.bytes - t * s.tile;
-  left = left < 0 ? 0 : left > INT32_MAX ? INT32_MAX : left;
-  const char* p = s.base + (left ? t * s.tile : 0);
-  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)left, 0x00027000);
+// The rows from `off` bytes on; empty where not `live`.
+__device__ inline __amdgpu_buffer_rsrc_t rows_from(const Stream& s,
+                                                   int64_t off, bool live) {
+  const int64_t left = live ? s.bytes - off : 0;
+  const int size = left > INT32_MAX ? INT32_MAX : left < 0 ? 0 : (int)left;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(s.base + off), 0, size,
+                                           0x00027000);
 }
 
 // One product: dy in tiles of kTM rows, `tiles` in all; x' starts again
@@ -114,7 +118,9 @@ struct Product {
   int ntiles, ktiles;
   int64_t n, k;
   void* dw;
+  void* db;                // null: not wanted
   float* partial;          // [slices, n, k] where slices > 1
+  float* bias_partial;     // [slices, n] where slices > 1
 };
 
 // The workgroup's tile of dW.  Workgroups go to the 8 XCDs in turn; each XCD
@@ -128,6 +134,31 @@ __device__ inline void pick_tile(const Product& p, int& tn, int& tk) {
   const int high = p.ntiles - strip * 8 < 8 ? p.ntiles - strip * 8 : 8;
   tn = strip * 8 + in % high;
   tk = in / high;
+}
+
+// The order of a step's instructions: the next step's fragments are read
+// between the first half of the matrix instructions, so that they are there
+// when that step begins, and the next tile is written and the one after
+// loaded between the others.  Left to itself the compiler gathers the loads
+// at the tile's end, next to the waits for them.
+template <int FN, int FK>
+__device__ inline void order_step(bool staging) {
+  constexpr int kMfma = 0x8, kVmem = 0x20, kRead = 0x100, kWrite = 0x200;
+  constexpr int kCount = FN * FK, kHalf = kCount / 2;
+  constexpr int kReads = 2 * (FN + FK) / kHalf;
+#pragma unroll
+  for (int i = 0; i < kHalf; i++) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, kReads, 0);
+  }
+#pragma unroll
+  for (int i = kHalf; i < kCount; i++) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+    if (!staging) continue;
+    __builtin_amdgcn_sched_group_barrier(kWrite, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kVmem, 2, 0);
+  }
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // T: bf16 or fp16, the operands' type.  O: the type of dW.  A wave computes
@@ -180,11 +211,19 @@ void act8_wgrad_kernel(Product p) {
   uint2v hx[kPassK];
   uint32_t he[kPassK];
   __amdgpu_buffer_rsrc_t by, bx, be;
-  auto aim = [&](int t) {  // the descriptors at tile t, past the end: empty
-    by = at_tile(p.dy, t < t1 ? t : INT32_MAX);
-    const int tx = t < t1 ? t % p.xtiles : INT32_MAX;
-    bx = at_tile(p.codes, tx);
-    be = at_tile(p.exps, tx);
+  // the descriptors of tile ta, and on to the next; past the end: empty
+  int ta = t0, tx = t0 % p.xtiles;
+  int64_t oy = t0 * p.dy.tile, ox = tx * p.codes.tile, oe = tx * p.exps.tile;
+  auto aim = [&]() {
+    by = rows_from(p.dy, oy, ta < t1);
+    bx = rows_from(p.codes, ox, ta < t1);
+    be = rows_from(p.exps, oe, ta < t1);
+    const bool wrap = ++tx == p.xtiles;
+    ta++;
+    oy += p.dy.tile;
+    ox = wrap ? 0 : ox + p.codes.tile;
+    oe = wrap ? 0 : oe + p.exps.tile;
+    tx = wrap ? 0 : tx;
   };
   auto load_y = [&](int i) {
     hy[i] = __builtin_amdgcn_raw_buffer_load_b128(by, gy,
@@ -223,54 +262,74 @@ void act8_wgrad_kernel(Product p) {
       ax[to][i] = read_fragment<kTK>(&lds[buf + fx[i] + step * 16 * kTK]);
   };
 
-  aim(t0);
+  // A step's share of the rows: those in registers go to `write` (LDS), if
+  // that is not negative, and the same of the tile aimed at take their place.
+  auto stage = [&](int step, int write, auto&& use_row) {
 #pragma unroll
-  for (int i = 0; i < kPassN; i++) load_y(i);
+    for (int i = 0; i < kPassN; i++)
+      if (i * (kSteps - 1) / kPassN == step) {
+        if (write >= 0) {
+          write_y(write, i);
+          use_row(i);
+        }
+        load_y(i);
+      }
 #pragma unroll
-  for (int i = 0; i < kPassK; i++) load_x(i);
-  aim(t0 + 1);
+    for (int i = 0; i < kPassK; i++)
+      if (i * (kSteps - 1) / kPassK == step) {
+        if (write >= 0) write_x(write, i);
+        load_x(i);
+      }
+  };
+
+  // The workgroups of the first column of tiles add dy's rows up for db as
+  // they pass through their registers: a pass over dy of its own took 52 us
+  // where the product takes 920.
+  float8 sum = 0.f;
+  auto add_row = [&](int i) {
+    sum += widen(__builtin_bit_cast(typename RowVec<T>::type, hy[i]));
+  };
+  aim();
 #pragma unroll
-  for (int i = 0; i < kPassN; i++) {
-    write_y(0, i);
-    load_y(i);
-  }
+  for (int s = 0; s < kSteps - 1; s++) stage(s, -1, add_row);
+  aim();
 #pragma unroll
-  for (int i = 0; i < kPassK; i++) {
-    write_x(0, i);
-    load_x(i);
+  for (int s = 0; s < kSteps - 1; s++) {
+    stage(s, 0, add_row);
+    __builtin_amdgcn_sched_barrier(0);
   }
   __syncthreads();
   read_step(0, 0, 0);
 
-  int cur = 0;  // where in LDS the tile at work begins
-  for (int t = t0; t < t1; t++) {
-    const int nxt = kTile - cur;
-    aim(t + 2);
+  auto all_tiles = [&](auto with_bias) {
+    constexpr bool kBias = decltype(with_bias)::value;
+    int cur = 0;  // where in LDS the tile at work begins
+    for (int t = t0; t < t1; t++) {
+      const int nxt = kTile - cur;
+      aim();
 #pragma unroll
-    for (int s = 0; s < kSteps; s++) {
-      if (s == kSteps - 1) __syncthreads();
-      read_step(s == kSteps - 1 ? nxt : cur, (s + 1) % kSteps, (s + 1) % 2);
-      // the next tile's rows into LDS, spread over the steps but the last
+      for (int s = 0; s < kSteps; s++) {
+        if (s == kSteps - 1) __syncthreads();
+        read_step(s == kSteps - 1 ? nxt : cur, (s + 1) % kSteps, (s + 1) % 2);
+        // the next tile's rows into LDS, spread over the steps but the last
+        if (s < kSteps - 1)
+          stage(s, nxt, [&](int i) {
+            if (kBias) add_row(i);
+          });
 #pragma unroll
-      for (int i = 0; i < kPassN; i++)
-        if (i * (kSteps - 1) / kPassN == s) {
-          write_y(nxt, i);
-          load_y(i);
-        }
+        for (int i = 0; i < FN; i++)
 #pragma unroll
-      for (int i = 0; i < kPassK; i++)
-        if (i * (kSteps - 1) / kPassK == s) {
-          write_x(nxt, i);
-          load_x(i);
-        }
-#pragma unroll
-      for (int i = 0; i < FN; i++)
-#pragma unroll
-        for (int j = 0; j < FK; j++)
-          acc[i][j] = mfma<T>(ay[s % 2][i], ax[s % 2][j], acc[i][j]);
+          for (int j = 0; j < FK; j++)
+            acc[i][j] = mfma<T>(ay[s % 2][i], ax[s % 2][j], acc[i][j]);
+        order_step<FN, FK>(s < kSteps - 1);
+      }
+      cur = nxt;
     }
-    cur = nxt;
-  }
+  };
+  if (p.db && tk == 0)
+    all_tiles(std::true_type());
+  else
+    all_tiles(std::false_type());
 
   // Out through LDS, 32 rows of a wave at a time, so that a lane writes 8
   // neighbours of a row: written straight from where the matrix instructions
@@ -280,6 +339,23 @@ void act8_wgrad_kernel(Product p) {
   constexpr int kPitch = FK * 32 + 8;
   static_assert(4 * 32 * kPitch * 2 <= 2 * kTile, "LDS");
   __syncthreads();
+  if (p.db && tk == 0) {
+    // columns' sums of the threads that had the same ones, in a fixed order
+    float* part = (float*)lds;
+    *(float8*)&part[ry * kTN + cy] = sum;
+    __syncthreads();
+    const int64_t n = n0 + threadIdx.x;
+    if (threadIdx.x < kTN && n < p.n) {
+      float v = 0.f;
+      for (int r = 0; r < kThreads * 8 / kTN; r++)
+        v += part[r * kTN + threadIdx.x];
+      if (p.slices > 1)
+        p.bias_partial[blockIdx.y * p.n + n] = v;
+      else
+        ((O*)p.db)[n] = (O)v;
+    }
+    __syncthreads();
+  }
   float* out = (float*)lds + wave * 32 * kPitch;
   const int er = lane / (FK * 4), ec = lane % (FK * 4) * kVec;
   const int64_t ek = k0 + wk + ec;
@@ -309,18 +385,23 @@ void act8_wgrad_kernel(Product p) {
   }
 }
 
-// dW from the slices' sums, in their order.
+// dW and db from the slices' sums, in their order.
 template <typename O>
 __global__ __launch_bounds__(kThreads) void wgrad_join_kernel(
-    const float* partial, int slices, int64_t count, O* dw) {
-  for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kVec;
-       i < count; i += (int64_t)gridDim.x * kThreads * kVec) {
+    const float* partial, const float* bias, int slices, int64_t count,
+    int64_t n, O* dw, O* db) {
+  const int64_t step = (int64_t)gridDim.x * kThreads * kVec;
+  const int64_t first = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kVec;
+  auto join = [&](const float* parts, int64_t i, int64_t count, O* out) {
     const int m = (int)(count - i < kVec ? count - i : kVec);
     float8 v = 0.f;
-    for (int s = 0; s < slices; s++)
-      v += load_upto(partial + s * count + i, m);
-    store_upto(dw + i, v, m);
-  }
+#pragma unroll 4
+    for (int s = 0; s < slices; s++) v += load_upto(parts + s * count + i, m);
+    store_upto(out + i, v, m);
+  };
+  for (int64_t i = first; i < count; i += step) join(partial, i, count, dw);
+  if (db)
+    for (int64_t i = first; i < n; i += step) join(bias, i, n, db);
 }
 
 // Gradients that the product cannot read as they are, laid out anew: rows
@@ -362,50 +443,53 @@ __global__ __launch_bounds__(kThreads) void layout_kernel(
   }
 }
 
-// Column sums of dy: strips of rows first, then the strips in their order.
-constexpr int kSumCols = 64, kSumLanes = 16;
-
-template <typename T>
-__global__ __launch_bounds__(kSumCols* kSumLanes) void column_strip_kernel(
-    const T* dy, int64_t dstride, int64_t m, int64_t n, int64_t strip_rows,
-    float* strips) {
-  __shared__ float part[kSumLanes][kSumCols];
-  const int c = threadIdx.x % kSumCols, s = threadIdx.x / kSumCols;
-  const int64_t col = (int64_t)blockIdx.x * kSumCols + c;
-  const int64_t begin = blockIdx.y * strip_rows;
-  const int64_t end = begin + strip_rows < m ? begin + strip_rows : m;
-  float sum = 0.f;
-  if (col < n) {
-#pragma unroll 8
-    for (int64_t r = begin + s; r < end; r += kSumLanes)
-      sum += (float)dy[r * dstride + col];
-  }
-  part[s][c] = sum;
-  __syncthreads();
-  if (s || col >= n) return;
-  for (int i = 1; i < kSumLanes; i++) sum += part[i][c];
-  strips[blockIdx.y * n + col] = sum;
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void column_join_kernel(
-    const float* strips, int count, int64_t n, T* db) {
-  const int64_t col = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (col >= n) return;
-  float sum = 0.f;
-#pragma unroll 8
-  for (int i = 0; i < count; i++) sum += strips[i * n + col];
-  db[col] = (T)sum;
-}
-
 struct Plan {
   bool big, laid_out;
   int planes, slices, slice_tiles, xtiles, ntiles, ktiles;
-  int64_t pitch, strip_rows, strips;
-  size_t laid_bytes, partial_bytes, strip_bytes;
+  int64_t pitch;
+  size_t laid_bytes, partial_bytes, bias_bytes;
 };
 
 size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
+
+// The tiles' shape and the number of slices that the rows are cut in, by the
+// time that they take, in us, from measurements of bf16 products with 64 to
+// 16384 rows and 64 to 8192 columns (the model is within 15% of them).
+//
+// Tiles of 256 by 256, one workgroup to a compute unit, need half of the LDS
+// reads that tiles of 128 by 128 do for the same work (1.45 us for 64 rows, or
+// 0.36 for a quarter of it, against 0.62 alone and 1.05 for two that share a
+// compute unit), but leave more of a small dW's edge empty and cut it in
+// fewer pieces: 2048 x 2048 x 2048 takes 27 us with the small ones and 41 with
+// the large, 4096 x 4096 x 4096 150 and 113.  Slices fill compute units that
+// too few tiles leave idle and cost a second pass over their sums: 16384 x
+// 256 x 256 takes 160 us in one slice and 21 in 16.
+void pick_shape(const Act8Wgrad& a, Plan& p) {
+  const int64_t tiles = (int64_t)p.planes * p.xtiles;
+  double best = 0;
+  for (int big = 0; big < 2; big++) {
+    const int size = big ? 256 : 128;
+    const int64_t nt = (a.n + size - 1) / size, kt = (a.k + size - 1) / size;
+    for (int64_t cut = 1; cut <= 512 && cut <= tiles;
+         cut += 1 + cut / 16) {
+      const int64_t each = (tiles + cut - 1) / cut;
+      if ((tiles + each - 1) / each != cut) continue;
+      const double groups = (double)nt * kt * cut;
+      if (cut > 1 && groups > 1024) break;
+      const double rounds = ceil(groups / (big ? 256 : 512));
+      const double tile = big ? 1.45 : groups > 256 ? 1.05 : 0.62;
+      double t = rounds * (each * tile + (big ? 9 : 5));
+      if (cut > 1) t += 4 + cut * (double)a.n * a.k * 1e-6;
+      if (best > 0 && t >= best) continue;
+      best = t;
+      p.big = big;
+      p.ntiles = (int)nt;
+      p.ktiles = (int)kt;
+      p.slices = (int)cut;
+      p.slice_tiles = (int)each;
+    }
+  }
+}
 
 Plan plan_of(const Act8Wgrad& a) {
   Plan p = {};
@@ -418,28 +502,10 @@ Plan plan_of(const Act8Wgrad& a) {
   if (p.laid_out)
     p.laid_bytes =
         round256((size_t)p.planes * p.xtiles * kTM * p.pitch * 2);
-  // Tiles of 256 by 256 need half of the LDS reads that tiles of 128 by 128
-  // do for the same work, but leave more of a small dW's edge empty and cut
-  // it in fewer pieces.
-  p.big = a.n > 512 && a.k > 512;
-  const int size = p.big ? 256 : 128;
-  p.ntiles = (int)((a.n + size - 1) / size);
-  p.ktiles = (int)((a.k + size - 1) / size);
-  // Few tiles leave compute units idle: the rows are then cut in slices of
-  // at least four tiles.
-  const int64_t tiles = (int64_t)p.planes * p.xtiles;
-  const int64_t places = p.big ? 256 : 512;
-  int64_t slices = places / ((int64_t)p.ntiles * p.ktiles);
-  if (slices > tiles / 4) slices = tiles / 4;
-  if (slices < 1) slices = 1;
-  p.slice_tiles = (int)((tiles + slices - 1) / slices);
-  p.slices = (int)((tiles + p.slice_tiles - 1) / p.slice_tiles);
-  if (p.slices > 1)
+  pick_shape(a, p);
+  if (p.slices > 1) {
     p.partial_bytes = round256((size_t)p.slices * a.n * a.k * sizeof(float));
-  if (a.db) {
-    p.strip_rows = a.m > 256 * 1024 ? (a.m + 1023) / 1024 : 256;
-    p.strips = (a.m + p.strip_rows - 1) / p.strip_rows;
-    p.strip_bytes = round256((size_t)p.strips * a.n * sizeof(float));
+    p.bias_bytes = round256((size_t)p.slices * a.n * sizeof(float));
   }
   return p;
 }
@@ -464,7 +530,7 @@ uint32_t flat_grid(int64_t items) {
 size_t act8_wgrad_workspace(const Act8Wgrad& a) {
   if (a.m == 0 || a.n == 0 || a.k == 0) return 0;
   const Plan p = plan_of(a);
-  return p.laid_bytes + p.partial_bytes + p.strip_bytes;
+  return p.laid_bytes + p.partial_bytes + p.bias_bytes;
 }
 
 hipError_t act8_wgrad(const Act8Wgrad& a, hipStream_t stream) {
@@ -475,7 +541,6 @@ hipError_t act8_wgrad(const Act8Wgrad& a, hipStream_t stream) {
       plan.slices > 65535)
     return hipErrorInvalidValue;
   char* ws = (char*)a.workspace;
-  float* strips = (float*)(ws + plan.laid_bytes + plan.partial_bytes);
   const int64_t laid_rows = (int64_t)plan.xtiles * kTM;
   Product p = {};
   p.dpitch = (int)(plan.pitch * 2);
@@ -497,7 +562,9 @@ hipError_t act8_wgrad(const Act8Wgrad& a, hipStream_t stream) {
   p.n = a.n;
   p.k = a.k;
   p.dw = a.dw;
+  p.db = a.db;
   p.partial = (float*)(ws + plan.laid_bytes);
+  p.bias_partial = (float*)(ws + plan.laid_bytes + plan.partial_bytes);
   with_type(a.type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     using P = std::conditional_t<std::is_same_v<T, float>, bf16, T>;
@@ -506,21 +573,10 @@ hipError_t act8_wgrad(const Act8Wgrad& a, hipStream_t stream) {
              kThreads, stream, (const T*)a.dy, a.dstride, a.m, a.n, (P*)ws,
              laid_rows, plan.pitch);
     launch_product<P, T>(plan, p, stream);
-    if (plan.slices > 1) {
-      const int64_t count = a.n * a.k;
-      launch(wgrad_join_kernel<T>, flat_grid((count + kVec - 1) / kVec),
-             kThreads, stream, (const float*)p.partial, plan.slices, count,
-             (T*)a.dw);
-    }
-    if (a.db) {
-      const dim3 sums((uint32_t)((a.n + kSumCols - 1) / kSumCols),
-                      (uint32_t)plan.strips);
-      launch(column_strip_kernel<T>, sums, kSumCols * kSumLanes, stream,
-             (const T*)a.dy, a.dstride, a.m, a.n, plan.strip_rows, strips);
-      launch(column_join_kernel<T>,
-             (uint32_t)((a.n + kThreads - 1) / kThreads), kThreads, stream,
-             (const float*)strips, (int)plan.strips, a.n, (T*)a.db);
-    }
+    if (plan.slices > 1)
+      launch(wgrad_join_kernel<T>, flat_grid(a.n * a.k / kVec + 1), kThreads,
+             stream, (const float*)p.partial, (const float*)p.bias_partial,
+             plan.slices, a.n * a.k, a.n, (T*)a.dw, (T*)a.db);
   });
   return hipGetLastError();
 }
