@@ -56,9 +56,9 @@ __global__ __launch_bounds__(kBlock) void embedding_forward_kernel(
 // Sorting keeps few compute units busy and is bound by latency, so its
 // launches zero the table's gradient beside it: each takes a part of dW with
 // workgroups of its own.  Rows that get a sum are written twice that way, which
-// costs at most what reading their gradients does; looking up which rows have
-// no token instead (a binary search for each, then zeroing row by row) took
-// 120 us where this takes 60, at 50000 x 2048 and 16384 tokens.
+// costs at most what reading their gradients does.  (Looking up which rows have
+// no token, by binary search, and zeroing those together with the sums took
+// 160 us where this takes 70: a table of 50000 x 2048 bf16, 16384 tokens.)
 
 __device__ inline int32_t sort_key(const EmbeddingBwd& a, int64_t i) {
   const int64_t t = read_token(a.tokens, i, a.tok64);
@@ -69,6 +69,12 @@ struct Sorted {
   int32_t *key, *pos;
 };
 
+// The chunks where a run starts that crosses chunk borders (see below), in any
+// order, and how many there are.  The sort sets the number to 0.
+struct Starts {
+  int32_t *count, *chunk;
+};
+
 // A launch's part of the bytes to zero, in 16-byte pieces; the workgroups from
 // `first` on do it.  The last part takes the rest of fewer than 16 bytes.
 struct Zero {
@@ -77,29 +83,38 @@ struct Zero {
   uint32_t first;
 };
 
+constexpr int kZeroPieces = 4;  // of 16 bytes, for each thread
+
 template <int kThreads>
 __device__ inline bool zero_part(const Zero& z) {
   if (blockIdx.x < z.first) return false;
-  const int64_t id = (int64_t)(blockIdx.x - z.first) * kThreads + threadIdx.x;
-  const int64_t step = (int64_t)(gridDim.x - z.first) * kThreads;
+  const int64_t block = blockIdx.x - z.first;
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  for (int64_t i = z.begin + id; i < z.end; i += step) ((uint4*)z.p)[i] = zero;
-  if (id < z.rest) ((uint16_t*)z.p)[z.end * 8 + id] = 0;
+#pragma unroll
+  for (int j = 0; j < kZeroPieces; j++) {
+    const int64_t i =
+        z.begin + (block * kZeroPieces + j) * kThreads + threadIdx.x;
+    if (i < z.end) ((uint4*)z.p)[i] = zero;
+  }
+  if (block == 0 && threadIdx.x < z.rest)
+    ((uint16_t*)z.p)[z.end * 8 + threadIdx.x] = 0;
   return true;
 }
 
 // Few tokens: an element's place is the number of those before it in the
 // order, and these are counted directly.  64 elements to a workgroup, one to a
 // lane; its 16 waves count them against every 16th run of 64 others, which
-// pass through the lanes' registers.  n * n / 64 lane operations: 20 us at
-// 16384 tokens, where the passes of a radix sort take 28.
+// pass through the lanes' registers: 8 us for 2048 tokens and 22 for 8192,
+// where the four launches of a radix sort take 17 and 19.
 constexpr int kRankBlock = 1024;
 constexpr int kRankWaves = kRankBlock / kWave;
 
 __global__ __launch_bounds__(kRankBlock) void sort_rank_kernel(EmbeddingBwd a,
                                                                Sorted out,
+                                                               Starts starts,
                                                                Zero z) {
   if (zero_part<kRankBlock>(z)) return;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *starts.count = 0;
   __shared__ int counts[kRankWaves][kWave];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
@@ -133,15 +148,17 @@ __global__ __launch_bounds__(kRankBlock) void sort_rank_kernel(EmbeddingBwd a,
 }
 
 // More tokens: least-significant-digit radix sort.  Each pass counts the
-// digits of every tile of tokens, scans the counts and places the tile's
-// elements in order.  With few tiles each of them scans for itself and the
-// scan needs no launch.
+// digits of every tile of tokens and places the tile's elements in order.
+// The tiles are cut so that there are at most 64: each of them then adds up
+// the counts of all for itself, and their scan needs no launch of its own.
 constexpr int kSortBlock = 256;
 constexpr int kSortWaves = kSortBlock / kWave;
-constexpr int kTile = 1024;          // elements of a tile
-constexpr int kPerWave = kTile / kSortWaves;
 constexpr int kMaxBits = 10;         // of a digit: 1024 counters
-constexpr int64_t kOwnScan = 128;    // tiles
+constexpr int64_t kMaxTiles = 64;
+
+struct Tiles {
+  int64_t size, count;  // elements of a tile, a multiple of kSortBlock
+};
 
 __device__ inline int32_t pass_key(const EmbeddingBwd& a, const Sorted& in,
                                    int64_t i) {
@@ -150,15 +167,16 @@ __device__ inline int32_t pass_key(const EmbeddingBwd& a, const Sorted& in,
 
 // counts: [tiles, digits]
 __global__ __launch_bounds__(kSortBlock) void sort_count_kernel(
-    EmbeddingBwd a, Sorted in, int shift, int bits, uint32_t* counts, Zero z) {
+    EmbeddingBwd a, Sorted in, int shift, int bits, Tiles tiles,
+    uint32_t* counts, Zero z) {
   if (zero_part<kSortBlock>(z)) return;
   __shared__ uint32_t hist[1 << kMaxBits];
   const int bins = 1 << bits;
   for (int b = threadIdx.x; b < bins; b += kSortBlock) hist[b] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kTile;
-#pragma unroll
-  for (int j = threadIdx.x; j < kTile; j += kSortBlock)
+  const int64_t base = (int64_t)blockIdx.x * tiles.size;
+#pragma unroll 4
+  for (int64_t j = threadIdx.x; j < tiles.size; j += kSortBlock)
     if (base + j < a.n)
       atomicAdd(&hist[(pass_key(a, in, base + j) >> shift) & (bins - 1)], 1u);
   __syncthreads();
@@ -166,11 +184,9 @@ __global__ __launch_bounds__(kSortBlock) void sort_count_kernel(
     counts[(int64_t)blockIdx.x * bins + b] = hist[b];
 }
 
-// The sum of v over the threads before this one, and over all.
+// The sum of v over the threads before this one.
 template <int kThreads>
-__device__ inline uint32_t block_scan(uint32_t v, uint32_t* wave_total,
-                                      uint32_t& all) {
-  constexpr int kWaves = kThreads / kWave;
+__device__ inline uint32_t block_scan(uint32_t v, uint32_t* wave_total) {
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   uint32_t incl = v;
 #pragma unroll
@@ -178,41 +194,20 @@ __device__ inline uint32_t block_scan(uint32_t v, uint32_t* wave_total,
     const uint32_t up = __shfl_up(incl, o);
     if (lane >= o) incl += up;
   }
-  __syncthreads();
   if (lane == kWave - 1) wave_total[wave] = incl;
   __syncthreads();
   uint32_t before = 0;
-  all = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; w++) {
+  for (int w = 0; w < kThreads / kWave; w++)
     if (w < wave) before += wave_total[w];
-    all += wave_total[w];
-  }
   return before + incl - v;
 }
 
-// Where each tile places its first element of each digit, by one workgroup.
-__global__ __launch_bounds__(1024) void sort_scan_kernel(uint32_t* counts,
-                                                         int64_t tiles,
-                                                         int bins) {
-  __shared__ uint32_t wave_total[16];
-  const int b = threadIdx.x;
-  uint32_t total = 0, all;
-  if (b < bins)
-    for (int64_t t = 0; t < tiles; t++) total += counts[t * bins + b];
-  uint32_t run = block_scan<1024>(total, wave_total, all);
-  if (b >= bins) return;
-  for (int64_t t = 0; t < tiles; t++) {
-    const uint32_t c = counts[t * bins + b];
-    counts[t * bins + b] = run;
-    run += c;
-  }
-}
-
 __global__ __launch_bounds__(kSortBlock) void sort_place_kernel(
-    EmbeddingBwd a, Sorted in, Sorted out, int shift, int bits, int64_t tiles,
-    const uint32_t* counts, bool scanned, Zero z) {
+    EmbeddingBwd a, Sorted in, Sorted out, int shift, int bits, Tiles tiles,
+    const uint32_t* counts, Starts starts, Zero z) {
   if (zero_part<kSortBlock>(z)) return;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *starts.count = 0;
   // next[w][d]: where wave w places its next element of digit d
   __shared__ uint32_t next[kSortWaves][1 << kMaxBits];
   __shared__ uint32_t wave_total[kSortWaves];
@@ -221,57 +216,65 @@ __global__ __launch_bounds__(kSortBlock) void sort_place_kernel(
   for (int b = threadIdx.x; b < bins * kSortWaves; b += kSortBlock)
     next[b / bins][b % bins] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kTile + wave * kPerWave;
-  int32_t keys[kPerWave / kWave];
+  const int64_t own = tiles.size / kSortWaves;
+  const int64_t base = (int64_t)blockIdx.x * tiles.size + wave * own;
+#pragma unroll 4
+  for (int64_t j = lane; j < own; j += kWave)
+    if (base + j < a.n)
+      atomicAdd(
+          &next[wave][(pass_key(a, in, base + j) >> shift) & (bins - 1)], 1u);
+  __syncthreads();
+  // a thread takes four digits: those of the tiles before, and of all
+  const int b = threadIdx.x * 4;
+  uint4 mine = make_uint4(0, 0, 0, 0), whole = mine;
+  if (b < bins) {
+    // 16 loads at a time: one by one they would wait for each other
+    constexpr int kLoads = 16;
+    const int count = (int)tiles.count;
+    for (int t0 = 0; t0 < count; t0 += kLoads) {
+      uint4 c[kLoads];
 #pragma unroll
-  for (int j = 0; j < kPerWave / kWave; j++) {
-    const int64_t i = base + j * kWave + lane;
-    keys[j] = i < a.n ? pass_key(a, in, i) : 0;
-    if (i < a.n) atomicAdd(&next[wave][(keys[j] >> shift) & (bins - 1)], 1u);
-  }
-  // bins come four to a thread at most, in order
-  const int per = (bins + kSortBlock - 1) / kSortBlock;
-  uint32_t first[4], total = 0, all;
-#pragma unroll
-  for (int q = 0; q < 4; q++) {
-    const int b = threadIdx.x * per + q;
-    first[q] = 0;
-    if (q >= per || b >= bins) continue;
-    if (scanned) {
-      first[q] = counts[(int64_t)blockIdx.x * bins + b];
-    } else {
-      uint32_t mine = 0, whole = 0;
-#pragma unroll 8
-      for (int64_t t = 0; t < tiles; t++) {
-        const uint32_t c = counts[t * bins + b];
-        whole += c;
-        mine += t < (int64_t)blockIdx.x ? c : 0;
+      for (int i = 0; i < kLoads; i++) {
+        const int t = t0 + i < count ? t0 + i : count - 1;
+        c[i] = *(const uint4*)&counts[t * bins + b];
       }
-      first[q] = total + mine;
-      total += whole;
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) {
+        const uint32_t in_all = t0 + i < count ? ~0u : 0u;
+        const uint32_t in_mine = t0 + i < (int)blockIdx.x ? ~0u : 0u;
+        whole.x += c[i].x & in_all, mine.x += c[i].x & in_mine;
+        whole.y += c[i].y & in_all, mine.y += c[i].y & in_mine;
+        whole.z += c[i].z & in_all, mine.z += c[i].z & in_mine;
+        whole.w += c[i].w & in_all, mine.w += c[i].w & in_mine;
+      }
     }
   }
-  const uint32_t before = block_scan<kSortBlock>(total, wave_total, all);
+  const uint32_t before = block_scan<kSortBlock>(
+      whole.x + whole.y + whole.z + whole.w, wave_total);
+  if (b < bins) {
+    uint32_t run[4] = {before + mine.x, before + whole.x + mine.y,
+                       before + whole.x + whole.y + mine.z,
+                       before + whole.x + whole.y + whole.z + mine.w};
 #pragma unroll
-  for (int q = 0; q < 4; q++) {
-    const int b = threadIdx.x * per + q;
-    if (q >= per || b >= bins) continue;
-    uint32_t run = first[q] + (scanned ? 0 : before);
+    for (int q = 0; q < 4; q++)
 #pragma unroll
-    for (int w = 0; w < kSortWaves; w++) {
-      const uint32_t c = next[w][b];
-      next[w][b] = run;
-      run += c;
-    }
+      for (int w = 0; w < kSortWaves; w++) {
+        const uint32_t c = next[w][b + q];
+        next[w][b + q] = run[q];
+        run[q] += c;
+      }
   }
   __syncthreads();
   // Each wave takes its elements 64 at a time, in order; lanes with the
   // same digit find one another by one ballot for each bit.
-#pragma unroll
-  for (int j = 0; j < kPerWave / kWave; j++) {
-    const int64_t i = base + j * kWave + lane;
+  int32_t ahead = base + lane < a.n ? pass_key(a, in, base + lane) : 0;
+  for (int64_t j = lane; j < own; j += kWave) {
+    const int64_t i = base + j;
     const bool live = i < a.n;
-    const int32_t key = keys[j];
+    const int32_t key = ahead;
+    const int32_t pos = in.pos && live ? in.pos[i] : (int32_t)i;
+    const int64_t after = i + kWave;
+    if (j + kWave < own && after < a.n) ahead = pass_key(a, in, after);
     const int digit = (key >> shift) & (bins - 1);
     uint64_t same = __ballot(live);
     for (int b = 0; b < bits; b++) {
@@ -296,7 +299,7 @@ __global__ __launch_bounds__(kSortBlock) void sort_place_kernel(
     at += rank;
     if (live) {
       out.key[at] = key;
-      out.pos[at] = in.pos ? in.pos[i] : (int32_t)i;
+      out.pos[at] = pos;
     }
   }
 }
@@ -309,16 +312,16 @@ __global__ __launch_bounds__(kSortBlock) void sort_place_kernel(
 // the part that came from the chunk before in slot 0, one that starts here in
 // slot 1; embedding_join_kernel adds these in order.
 
-constexpr int kAhead = 8;      // rows in flight for each lane
-constexpr int kJoinAhead = 16;
-
 struct Chunks {
   int64_t size, count;  // positions of a chunk, and chunks
   int64_t tiles;        // of columns
   int tpr;
 };
 
-// The team's chunk and this lane's columns; false for those past the end.
+// The team's chunk, or false past the last, and the lane's columns: from `at`
+// on, as an offset of its own, so that a row may have any length.  Lanes at
+// and behind the row's end move back into it and write what their neighbours
+// write.
 template <bool kTiny>
 __device__ inline bool pick_chunk(const EmbeddingBwd& a, const Chunks& ch,
                                   int64_t& chunk, int64_t& at,
@@ -328,17 +331,17 @@ __device__ inline bool pick_chunk(const EmbeddingBwd& a, const Chunks& ch,
       (int64_t)blockIdx.x * (kBlock / ch.tpr) + threadIdx.x / ch.tpr;
   chunk = item / ch.tiles;
   at = ((item % ch.tiles) * ch.tpr + lane) * kVec;
-  if (chunk >= ch.count || at >= a.dim) return false;
-  // columns as an offset into the row, so that a row may have any length
-  const int64_t left = a.dim - at;
-  c = Cols<kTiny>(0, (int)(left < kVec ? left : kVec));
-  if (!kTiny && left < kVec) at = a.dim - kVec, c = Cols<kTiny>(0, kVec);
-  return true;
+  if (kTiny)
+    at = 0;
+  else if (at + kVec > a.dim)
+    at = a.dim - kVec;
+  c = Cols<kTiny>(0, kTiny ? (int)a.dim : kVec);
+  return chunk < ch.count;
 }
 
 template <typename D, typename W, bool kTiny>
 __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(
-    EmbeddingBwd a, Sorted s, Chunks ch, float* partial) {
+    EmbeddingBwd a, Sorted s, Chunks ch, Starts starts, float* partial) {
   int64_t chunk, at;
   Cols<kTiny> c;
   if (!pick_chunk(a, ch, chunk, at, c)) return;
@@ -348,15 +351,18 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(
   const int32_t after = p1 < a.n ? s.key[p1] : -1;
   const D* dout = (const D*)a.dout + at;
 
+  // Four rows in flight for each lane: with 8 or 16 the registers they take
+  // leave fewer waves (187, 204 and 456 us at 65536 rows of 4096 bf16).
+  constexpr int kAhead = 4;
   float8 acc = 0.f;
-  int32_t cur = s.key[p0];
-  bool head = cur == before;  // the run now summed began in a chunk before
+  int32_t run = s.key[p0];
+  bool head = run == before;  // the run now summed began in a chunk before
   auto flush = [&](bool tail) {
-    if (cur >= a.vocab) return;
+    if (run >= a.vocab) return;
     if (head || tail)
       c.store(partial + (chunk * 2 + (head ? 0 : 1)) * a.dim + at, acc);
     else
-      c.store((W*)a.dweight + (int64_t)cur * a.dim + at, acc * a.scale);
+      c.store((W*)a.dweight + (int64_t)run * a.dim + at, acc * a.scale);
   };
   for (int64_t p = p0; p < p1; p += kAhead) {
     typename RowVec<D>::type row[kAhead];
@@ -371,48 +377,84 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(
 #pragma unroll
     for (int j = 0; j < kAhead; j++) {
       if (p + j >= p1) break;
-      if (key[j] != cur) {
+      if (key[j] != run) {
         flush(false);
-        cur = key[j];
+        run = key[j];
         head = false;
-        acc = widen(row[j]);
-      } else {
-        acc += widen(row[j]);
+        acc = 0.f;
       }
+      acc += widen(row[j]);
     }
   }
-  flush(cur == after);
+  flush(run == after);
+  if (run == after && run < a.vocab && !head && at == 0)
+    starts.chunk[atomicAdd(starts.count, 1)] = (int32_t)chunk;
 }
 
-// A run that crosses chunk borders, summed from its parts in their order by
-// the team of the chunk where it starts.
+// The runs that cross chunk borders, each summed from its parts by one
+// workgroup for a tile of columns: its threads look for the run's end
+// together, each of its teams adds up every so many of the parts, and the
+// teams' sums are added in their order.
+constexpr int kJoinBlock = 1024;
+
 template <typename W, bool kTiny>
-__global__ __launch_bounds__(kBlock) void embedding_join_kernel(
-    EmbeddingBwd a, Sorted s, Chunks ch, const float* partial) {
-  int64_t chunk, at;
-  Cols<kTiny> c;
-  if (!pick_chunk(a, ch, chunk, at, c) || chunk + 1 >= ch.count) return;
-  const int64_t p1 = (chunk + 1) * ch.size;
-  const int32_t key = s.key[p1 - 1];
-  if (key >= a.vocab || s.key[p1] != key) return;   // nothing crosses here
-  const int64_t p0 = p1 - ch.size;
-  if (p0 && s.key[p0] == key && s.key[p0 - 1] == key) return;  // not its start
-  float8 acc = c.load(partial + (chunk * 2 + 1) * a.dim + at);
-  // chunks that begin with the key hold a part in slot 0
-  for (int64_t q = chunk + 1;; q += kJoinAhead) {
-    float8 part[kJoinAhead];
-    bool more = true;
-#pragma unroll
-    for (int j = 0; j < kJoinAhead; j++) {
-      more = more && q + j < ch.count && s.key[(q + j) * ch.size] == key;
-      part[j] = 0.f;
-      if (more) part[j] = c.load(partial + (q + j) * 2 * a.dim + at);
+__global__ __launch_bounds__(kJoinBlock) void embedding_join_kernel(
+    EmbeddingBwd a, Sorted s, Chunks ch, Starts starts, const float* partial) {
+  __shared__ int wave_end[kJoinBlock / kWave];
+  __shared__ float joint[kJoinBlock * kVec];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int tpr = ch.tpr, teams = kJoinBlock / tpr;
+  const int team = threadIdx.x / tpr, in = threadIdx.x % tpr;
+  const int64_t items = *starts.count * ch.tiles;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t chunk = starts.chunk[item / ch.tiles];
+    const int32_t key = s.key[(chunk + 1) * ch.size - 1];
+    // chunks that begin with the key hold a part in slot 0
+    int64_t parts = 1;
+    for (bool more = true; more;) {
+      const int64_t q = chunk + parts + threadIdx.x;
+      const uint64_t differ =
+          __ballot(q >= ch.count || s.key[q * ch.size] != key);
+      if (lane == 0)
+        wave_end[wave] = differ ? __ffsll((long long)differ) - 1 : kWave;
+      __syncthreads();
+      for (int w = 0; more && w < kJoinBlock / kWave; w++) {
+        parts += wave_end[w];
+        more = wave_end[w] == kWave;
+      }
+      __syncthreads();
     }
+    int64_t at = ((item % ch.tiles) * tpr + in) * kVec;
+    if (kTiny)
+      at = 0;
+    else if (at + kVec > a.dim)
+      at = a.dim - kVec;
+    const Cols<kTiny> c(0, kTiny ? (int)a.dim : kVec);
+    constexpr int kAhead = 4;
+    float8 acc = 0.f;
+    for (int64_t j = team; j < parts; j += teams * kAhead) {
+      float8 part[kAhead];
 #pragma unroll
-    for (int j = 0; j < kJoinAhead; j++) acc += part[j];
-    if (!more) break;
+      for (int i = 0; i < kAhead; i++) {
+        const int64_t k = j + i * teams;  // part 0 is in slot 1
+        part[i] = 0.f;
+        if (k < parts)
+          part[i] =
+              c.load(partial + ((chunk + k) * 2 + (k ? 0 : 1)) * a.dim + at);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; i++) acc += part[i];
+    }
+    *(float8*)&joint[threadIdx.x * kVec] = acc;
+    __syncthreads();
+    if (team == 0) {
+      const int used = parts < teams ? (int)parts : teams;
+      for (int t = 1; t < used; t++)
+        acc += *(const float8*)&joint[(t * tpr + in) * kVec];
+      c.store((W*)a.dweight + (int64_t)key * a.dim + at, acc * a.scale);
+    }
+    __syncthreads();
   }
-  c.store((W*)a.dweight + (int64_t)key * a.dim + at, acc * a.scale);
 }
 
 // HIP counts a launch's threads in 32 bits.
@@ -434,7 +476,7 @@ size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
 
 struct Layout {
   Chunks chunks;
-  size_t sorted, counts, total;
+  size_t sorted, counts, starts, total;
 };
 
 Layout layout(int64_t dim, int64_t n) {
@@ -442,21 +484,22 @@ Layout layout(int64_t dim, int64_t n) {
   l.chunks.tpr = team_size(dim);
   const int64_t width = (int64_t)l.chunks.tpr * kVec;
   l.chunks.tiles = (dim + width - 1) / width;
-  // Chunks of 64 positions leave little to join; with few tokens they are
-  // shorter, for about 1024 teams.
+  // Chunks of 64 positions leave little to join; with fewer tokens or columns
+  // they are shorter, so that each compute unit has 2048 lanes at work.
   l.chunks.size = 64;
-  while (l.chunks.size > 8 && n * l.chunks.tiles / l.chunks.size < 1024)
+  while (l.chunks.size > 8 &&
+         n * l.chunks.tiles * l.chunks.tpr / l.chunks.size < 256 * 2048)
     l.chunks.size /= 2;
   l.chunks.count = (n + l.chunks.size - 1) / l.chunks.size;
   l.sorted = round256((size_t)n * 4);
-  const size_t tiles = (size_t)((n + kTile - 1) / kTile);
-  l.counts = round256((tiles << kMaxBits) * 4);
-  l.total = 4 * l.sorted + l.counts +
+  l.counts = round256((kMaxTiles << kMaxBits) * 4);
+  l.starts = round256((size_t)(l.chunks.count + 1) * 4);
+  l.total = 4 * l.sorted + l.counts + l.starts +
             round256((size_t)l.chunks.count * 2 * (size_t)dim * 4);
   return l;
 }
 
-constexpr int64_t kRankMost = 16384;  // tokens that are sorted by counting
+constexpr int64_t kRankMost = 8192;  // tokens that are sorted by counting
 
 // Cuts the zeroing of dW in equal parts over `launches`.
 struct Zeroing {
@@ -467,9 +510,9 @@ struct Zeroing {
     const int64_t pieces = bytes / 16;
     Zero z = {p, pieces * i / launches, pieces * (i + 1) / launches,
               i + 1 == launches ? bytes % 16 / 2 : 0, (uint32_t)first};
-    const int64_t want = (z.end - z.begin + threads * 4 - 1) / (threads * 4);
-    const int64_t most = 256 * 2048 / threads;
-    grid = (uint32_t)(first + (want < 1 ? 1 : want < most ? want : most));
+    const int64_t each = (int64_t)threads * kZeroPieces;
+    const int64_t want = (z.end - z.begin + each - 1) / each;
+    grid = (uint32_t)(first + (want < 1 ? 1 : want));
     return z;
   }
 };
@@ -502,13 +545,18 @@ hipError_t embedding_backward(const EmbeddingBwd& a, hipStream_t stream) {
   const Chunks& ch = l.chunks;
   const int64_t teams = kBlock / ch.tpr;
   const int64_t blocks = (ch.count * ch.tiles + teams - 1) / teams;
-  if (blocks > kMaxBlocks) return hipErrorInvalidValue;
+  // the largest launches: the sums', and one that zeroes a part of dW
+  const int64_t zeros = a.vocab * a.dim / (kSortBlock * kZeroPieces * 4);
+  if (blocks > kMaxBlocks || zeros > kMaxBlocks / 2)
+    return hipErrorInvalidValue;
   char* ws = (char*)a.workspace;
   Sorted buf[2];
   buf[0] = {(int32_t*)ws, (int32_t*)(ws + l.sorted)};
   buf[1] = {(int32_t*)(ws + 2 * l.sorted), (int32_t*)(ws + 3 * l.sorted)};
   uint32_t* counts = (uint32_t*)(ws + 4 * l.sorted);
-  float* partial = (float*)(ws + 4 * l.sorted + l.counts);
+  int32_t* first = (int32_t*)(ws + 4 * l.sorted + l.counts);
+  const Starts starts = {first, first + 1};
+  float* partial = (float*)(ws + 4 * l.sorted + l.counts + l.starts);
 
   Zeroing zero = {a.dweight,
                   a.vocab * a.dim * (a.wtype == ElemType::kF32 ? 4 : 2), 1};
@@ -518,24 +566,26 @@ hipError_t embedding_backward(const EmbeddingBwd& a, hipStream_t stream) {
     const int64_t own = (a.n + kWave - 1) / kWave;
     const Zero z = zero.part(0, own, kRankBlock, grid);
     sorted = buf[0];
-    launch(sort_rank_kernel, grid, kRankBlock, stream, a, sorted, z);
+    launch(sort_rank_kernel, grid, kRankBlock, stream, a, sorted,
+           starts, z);
   } else {
     const int bits = key_bits(a.vocab);
     const int passes = (bits + kMaxBits - 1) / kMaxBits;
-    const int digit = (bits + passes - 1) / passes;
-    const int64_t tiles = (a.n + kTile - 1) / kTile;
+    // at least 4 bits: the placing reads the counts of four digits at once
+    const int even = (bits + passes - 1) / passes, digit = even < 4 ? 4 : even;
+    Tiles tiles;
+    tiles.size = (a.n + kMaxTiles - 1) / kMaxTiles;
+    tiles.size = (tiles.size + kSortBlock - 1) / kSortBlock * kSortBlock;
+    tiles.count = (a.n + tiles.size - 1) / tiles.size;
     zero.launches = 2 * passes;
     for (int p = 0; p < passes; p++) {
       const Sorted out = buf[p & 1];
-      const Zero zc = zero.part(2 * p, tiles, kSortBlock, grid);
+      const Zero zc = zero.part(2 * p, tiles.count, kSortBlock, grid);
       launch(sort_count_kernel, grid, kSortBlock, stream, a, sorted, p * digit,
-             digit, counts, zc);
-      if (tiles > kOwnScan)
-        launch(sort_scan_kernel, 1, 1024, stream, counts, tiles, 1 << digit);
-      const Zero zp = zero.part(2 * p + 1, tiles, kSortBlock, grid);
+             digit, tiles, counts, zc);
+      const Zero zp = zero.part(2 * p + 1, tiles.count, kSortBlock, grid);
       launch(sort_place_kernel, grid, kSortBlock, stream, a, sorted, out,
-             p * digit, digit, tiles, (const uint32_t*)counts,
-             tiles > kOwnScan, zp);
+             p * digit, digit, tiles, (const uint32_t*)counts, starts, zp);
       sorted = out;
     }
   }
@@ -548,11 +598,14 @@ hipError_t embedding_backward(const EmbeddingBwd& a, hipStream_t stream) {
       with_type(a.dtype, [&](auto* d) {
         using D = std::remove_pointer_t<decltype(d)>;
         launch(embedding_sum_kernel<D, W, kTiny>, (uint32_t)blocks, kBlock,
-               stream, a, sorted, ch, partial);
+               stream, a, sorted, ch, starts, partial);
       });
       if (ch.count > 1)
-        launch(embedding_join_kernel<W, kTiny>, (uint32_t)blocks, kBlock,
-               stream, a, sorted, ch, (const float*)partial);
+        launch(embedding_join_kernel<W, kTiny>,
+               (uint32_t)(ch.count * ch.tiles < 512 ? ch.count * ch.tiles
+                                                    : 512),
+               kJoinBlock, stream, a, sorted, ch, starts,
+               (const float*)partial);
     };
     if (a.dim < kVec)
       sums(std::true_type());
