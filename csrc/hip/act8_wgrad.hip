@@ -89,23 +89,18 @@ __device__ inline short8v read_fragment(const short* p) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// Memory that is read a tile of rows at a time.  Reads behind its end give
-// zeros (the hardware checks them against the descriptor's size), so the
+// Memory that is read a tile of rows at a time.  Reads behind a tile's bytes
+// give zeros (the hardware checks them against the descriptor's size), so the
 // last tile needs no conditions; those behind a row's end give the next
 // row's values, which only reach columns that are not written.
 struct Stream {
   const char* base;
-  int64_t bytes;      // in all
-  int64_t tile;       // from one tile to the next
+  int64_t tile;    // bytes from one tile to the next
+  int full, tail;  // bytes of a tile, and of the last
 };
 
-// The rows from `off` bytes on; empty where not `live`.
-__device__ inline __amdgpu_buffer_rsrc_t rows_from(const Stream& s,
-                                                   int64_t off, bool live) {
-  const int64_t left = live ? s.bytes - off : 0;
-  const int size = left > INT32_MAX ? INT32_MAX : left < 0 ? 0 : (int)left;
-  return __builtin_amdgcn_make_buffer_rsrc((void*)(s.base + off), 0, size,
-                                           0x00027000);
+__device__ inline __amdgpu_buffer_rsrc_t descriptor(const char* p, int size) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, size, 0x00027000);
 }
 
 // One product: dy in tiles of kTM rows, `tiles` in all; x' starts again
@@ -143,7 +138,7 @@ __device__ inline void pick_tile(const Product& p, int& tn, int& tk) {
 // at the tile's end, next to the waits for them.
 template <int FN, int FK>
 __device__ inline void order_step(bool staging) {
-  constexpr int kMfma = 0x8, kVmem = 0x20, kRead = 0x100, kWrite = 0x200;
+  constexpr int kMfma = 0x8, kScalar = 0x4, kVmem = 0x20, kRead = 0x100, kWrite = 0x200;
   constexpr int kCount = FN * FK, kHalf = kCount / 2;
   constexpr int kReads = 2 * (FN + FK) / kHalf;
 #pragma unroll
@@ -154,7 +149,10 @@ __device__ inline void order_step(bool staging) {
 #pragma unroll
   for (int i = kHalf; i < kCount; i++) {
     __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-    if (!staging) continue;
+    if (!staging) {
+      __builtin_amdgcn_sched_group_barrier(kScalar, 32 / kHalf, 0);
+      continue;
+    }
     __builtin_amdgcn_sched_group_barrier(kWrite, 1, 0);
     __builtin_amdgcn_sched_group_barrier(kVmem, 2, 0);
   }
@@ -213,17 +211,22 @@ void act8_wgrad_kernel(Product p) {
   __amdgpu_buffer_rsrc_t by, bx, be;
   // the descriptors of tile ta, and on to the next; past the end: empty
   int ta = t0, tx = t0 % p.xtiles;
-  int64_t oy = t0 * p.dy.tile, ox = tx * p.codes.tile, oe = tx * p.exps.tile;
+  const char* py = p.dy.base + t0 * p.dy.tile;
+  const char* px = p.codes.base + tx * p.codes.tile;
+  const char* pe = p.exps.base + tx * p.exps.tile;
   auto aim = [&]() {
-    by = rows_from(p.dy, oy, ta < t1);
-    bx = rows_from(p.codes, ox, ta < t1);
-    be = rows_from(p.exps, oe, ta < t1);
-    const bool wrap = ++tx == p.xtiles;
+    const bool live = ta < t1, last = tx == p.xtiles - 1;
+    const int sy = ta == p.tiles - 1 ? p.dy.tail : p.dy.full;
+    const int sx = last ? p.codes.tail : p.codes.full;
+    const int se = last ? p.exps.tail : p.exps.full;
+    by = descriptor(py, live ? sy : 0);
+    bx = descriptor(px, live ? sx : 0);
+    be = descriptor(pe, live ? se : 0);
     ta++;
-    oy += p.dy.tile;
-    ox = wrap ? 0 : ox + p.codes.tile;
-    oe = wrap ? 0 : oe + p.exps.tile;
-    tx = wrap ? 0 : tx;
+    py += p.dy.tile;
+    tx = last ? 0 : tx + 1;
+    px = last ? p.codes.base : px + p.codes.tile;
+    pe = last ? p.exps.base : pe + p.exps.tile;
   };
   auto load_y = [&](int i) {
     hy[i] = __builtin_amdgcn_raw_buffer_load_b128(by, gy,
@@ -298,6 +301,7 @@ void act8_wgrad_kernel(Product p) {
     stage(s, 0, add_row);
     __builtin_amdgcn_sched_barrier(0);
   }
+  aim();
   __syncthreads();
   read_step(0, 0, 0);
 
@@ -306,7 +310,6 @@ void act8_wgrad_kernel(Product p) {
     int cur = 0;  // where in LDS the tile at work begins
     for (int t = t0; t < t1; t++) {
       const int nxt = kTile - cur;
-      aim();
 #pragma unroll
       for (int s = 0; s < kSteps; s++) {
         if (s == kSteps - 1) __syncthreads();
@@ -316,6 +319,8 @@ void act8_wgrad_kernel(Product p) {
           stage(s, nxt, [&](int i) {
             if (kBias) add_row(i);
           });
+        else
+          aim();  // the loads of the next tile's steps
 #pragma unroll
         for (int i = 0; i < FN; i++)
 #pragma unroll
@@ -545,14 +550,18 @@ hipError_t act8_wgrad(const Act8Wgrad& a, hipStream_t stream) {
   Product p = {};
   p.dpitch = (int)(plan.pitch * 2);
   p.cpitch = (int)a.pitch;
+  const int64_t last = (int64_t)(plan.xtiles - 1) * kTM;  // its first row
   p.dy.base = plan.laid_out ? ws : (const char*)a.dy;
-  p.dy.bytes = plan.laid_out
-                   ? plan.planes * laid_rows * plan.pitch * 2
-                   : ((a.m - 1) * a.dstride + a.n) * 2;
   p.dy.tile = (int64_t)kTM * plan.pitch * 2;
-  p.codes = {(const char*)a.codes, a.m * a.pitch, kTM * a.pitch};
-  p.exps = {(const char*)a.exps, a.m * a.pitch / kAct8Group,
-            kTM * a.pitch / kAct8Group};
+  p.dy.full = (int)p.dy.tile;
+  p.dy.tail = plan.laid_out
+                  ? p.dy.full
+                  : (int)(((a.m - last - 1) * a.dstride + a.n) * 2);
+  p.codes = {(const char*)a.codes, kTM * a.pitch, (int)(kTM * a.pitch),
+             (int)((a.m - last) * a.pitch)};
+  p.exps = {(const char*)a.exps, kTM * a.pitch / kAct8Group,
+            (int)(kTM * a.pitch / kAct8Group),
+            (int)((a.m - last) * a.pitch / kAct8Group)};
   p.xtiles = plan.xtiles;
   p.tiles = plan.planes * plan.xtiles;
   p.slices = plan.slices;
