@@ -7,6 +7,7 @@
 // come from torch's allocator, so calls may be captured into a graph.
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
@@ -58,6 +59,17 @@ void check_device(const Tensor& t, const Tensor& on, const char* op,
               t.device(), ", expected ", on.device());
 }
 
+// Whether a gradient will be asked of any of these.  Without one an operator
+// runs alone, keeps nothing and makes no graph.
+bool wants_grad(std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : tensors)
+    if (t && t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+const Tensor* get(const OptTensor& t) { return t ? &*t : nullptr; }
+
 void no_double_backward(const char* op) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op,
               ": its gradient cannot be differentiated again");
@@ -101,36 +113,39 @@ Tensor or_undefined(const OptTensor& t) { return t ? *t : Tensor(); }
 // ---------------------------------------------------------------------------
 // embedding
 
+Tensor lookup(const Tensor& weight, const Tensor& tok, double scale,
+              at::ScalarType out_type) {
+  const c10::OptionalDeviceGuard guard(weight.device());
+  const Tensor w = weight.stride(-1) == 1 ? weight : weight.contiguous();
+  c10::SmallVector<int64_t, 6> sizes(tok.sizes().begin(), tok.sizes().end());
+  sizes.push_back(weight.size(1));
+  Tensor out = at::empty(sizes, weight.options().dtype(out_type));
+  EmbeddingFwd a = {};
+  a.weight = w.data_ptr();
+  a.tokens = tok.data_ptr();
+  a.out = out.data_ptr();
+  a.vocab = w.size(0);
+  a.dim = w.size(1);
+  a.n = tok.numel();
+  a.wstride = w.stride(0);
+  a.scale = (float)scale;
+  a.tok64 = tok.scalar_type() == at::kLong;
+  a.wtype = elem(w.scalar_type());
+  a.otype = elem(out_type);
+  check_launch(embedding_forward(a, stream_of(w)), "embedding");
+  return out;
+}
+
 struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& weight,
-                        const Tensor& tokens, double scale, int64_t padding,
+                        const Tensor& tok, double scale, int64_t padding,
                         int64_t out_type) {
-    const c10::OptionalDeviceGuard guard(weight.device());
-    const Tensor w = weight.stride(-1) == 1 ? weight : weight.contiguous();
-    const Tensor tok = tokens.contiguous();
-    auto sizes = tokens.sizes().vec();
-    sizes.push_back(weight.size(1));
-    Tensor out = at::empty(
-        sizes, weight.options().dtype((at::ScalarType)out_type));
-    EmbeddingFwd a = {};
-    a.weight = w.data_ptr();
-    a.tokens = tok.data_ptr();
-    a.out = out.data_ptr();
-    a.vocab = w.size(0);
-    a.dim = w.size(1);
-    a.n = tok.numel();
-    a.wstride = w.stride(0);
-    a.scale = (float)scale;
-    a.tok64 = tok.scalar_type() == at::kLong;
-    a.wtype = elem(w.scalar_type());
-    a.otype = elem(out.scalar_type());
-    check_launch(embedding_forward(a, stream_of(w)), "embedding");
     ctx->save_for_backward({tok});
-    ctx->saved_data["vocab"] = w.size(0);
+    ctx->saved_data["vocab"] = weight.size(0);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
-    ctx->saved_data["type"] = (int64_t)w.scalar_type();
-    return out;
+    ctx->saved_data["type"] = (int64_t)weight.scalar_type();
+    return lookup(weight, tok, scale, (at::ScalarType)out_type);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -188,76 +203,102 @@ Tensor embedding(const Tensor& weight, const Tensor& tokens, double scale,
   }
   check_device(weight, weight, op, "weight");
   check_device(tokens, weight, op, "tokens");
-  return EmbeddingFn::apply(weight, tokens, scale, padding, (int64_t)out);
+  const Tensor tok = tokens.contiguous();
+  if (!wants_grad({&weight})) return lookup(weight, tok, scale, out);
+  return EmbeddingFn::apply(weight, tok, scale, padding, (int64_t)out);
 }
 
 // ---------------------------------------------------------------------------
 // gated residual norm
 
+struct NormArgs {
+  Tensor x, branch, gate, post, pre;  // undefined where not given
+  double residual_scale, branch_scale, eps;
+  Gate gmode;
+  int64_t group_rows;
+  bool want_h;
+};
+
+// y (where there is a branch) and h (where it is wanted); `stats`: [2, rows],
+// the reciprocals that the backward pass takes, or undefined.
+std::tuple<Tensor, Tensor> run_norm(const NormArgs& n, const Tensor& stats) {
+  const c10::OptionalDeviceGuard guard(n.x.device());
+  const Rows xr = as_rows(n.x);
+  NormFwd a = {};
+  a.rows = rows_of(n.x);
+  a.dim = n.x.size(-1);
+  a.x = xr.t.data_ptr();
+  a.xstride = xr.stride;
+  a.type = elem(n.x.scalar_type());
+  a.residual_scale = (float)n.residual_scale;
+  a.branch_scale = (float)n.branch_scale;
+  a.eps = (float)n.eps;
+  a.gmode = n.gmode;
+  a.group_rows = n.group_rows;
+  float* kept = stats.defined() ? stats.data_ptr<float>() : nullptr;
+  Tensor y, h;
+  Rows br;
+  if (n.branch.defined()) {
+    br = as_rows(n.branch);
+    a.branch = br.t.data_ptr();
+    a.bstride = br.stride;
+    y = at::empty(n.x.sizes(), n.x.options());
+    a.y = y.data_ptr();
+    if (n.gate.defined()) {
+      a.gate = n.gate.data_ptr();
+      a.gate32 = n.gate.scalar_type() == at::kFloat;
+    }
+    if (n.post.defined()) {
+      a.post = n.post.data_ptr();
+      a.post32 = n.post.scalar_type() == at::kFloat;
+      a.rbranch = kept;
+    }
+  }
+  if (n.want_h) {
+    h = at::empty(n.x.sizes(), n.x.options());
+    a.h = h.data_ptr();
+    a.ry = kept ? kept + a.rows : nullptr;
+    if (n.pre.defined()) {
+      a.pre = n.pre.data_ptr();
+      a.pre32 = n.pre.scalar_type() == at::kFloat;
+    }
+  }
+  check_launch(norm_forward(a, stream_of(n.x)), "residual norm");
+  return {y, h};
+}
+
 struct NormFn : torch::autograd::Function<NormFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x,
-                               const OptTensor& branch_, const OptTensor& gate_,
-                               const OptTensor& post_, const OptTensor& pre_,
+                               const OptTensor& branch, const OptTensor& gate,
+                               const OptTensor& post, const OptTensor& pre,
                                double residual_scale, double branch_scale,
                                double eps, int64_t gmode, int64_t group_rows,
                                bool want_h) {
-    const c10::OptionalDeviceGuard guard(x.device());
-    const Tensor branch = or_undefined(branch_), pre = or_undefined(pre_);
-    const Tensor gate = or_undefined(gate_), post = or_undefined(post_);
-    const Rows xr = as_rows(x);
-    NormFwd a = {};
-    a.rows = rows_of(x);
-    a.dim = x.size(-1);
-    a.x = xr.t.data_ptr();
-    a.xstride = xr.stride;
-    a.type = elem(x.scalar_type());
-    a.residual_scale = (float)residual_scale;
-    a.branch_scale = (float)branch_scale;
-    a.eps = (float)eps;
-    a.gmode = (Gate)gmode;
-    a.group_rows = group_rows;
-    const auto stats = x.options().dtype(at::kFloat);
-    Tensor y, h, rbranch, ry;
-    Rows br;
-    if (branch.defined()) {
-      br = as_rows(branch);
-      a.branch = br.t.data_ptr();
-      a.bstride = br.stride;
-      y = at::empty(x.sizes(), x.options());
-      a.y = y.data_ptr();
-      if (gate.defined()) {
-        a.gate = gate.data_ptr();
-        a.gate32 = gate.scalar_type() == at::kFloat;
-      }
-      if (post.defined()) {
-        a.post = post.data_ptr();
-        a.post32 = post.scalar_type() == at::kFloat;
-        rbranch = at::empty({a.rows}, stats);
-        a.rbranch = rbranch.data_ptr<float>();
-      }
-    }
-    if (want_h) {
-      h = at::empty(x.sizes(), x.options());
-      a.h = h.data_ptr();
-      ry = at::empty({a.rows}, stats);
-      a.ry = ry.data_ptr<float>();
-      if (pre.defined()) {
-        a.pre = pre.data_ptr();
-        a.pre32 = pre.scalar_type() == at::kFloat;
-      }
-    }
-    check_launch(norm_forward(a, stream_of(x)), "residual norm");
+    const NormArgs n = {x,
+                        or_undefined(branch),
+                        or_undefined(gate),
+                        or_undefined(post),
+                        or_undefined(pre),
+                        residual_scale,
+                        branch_scale,
+                        eps,
+                        (Gate)gmode,
+                        group_rows,
+                        want_h};
+    const Tensor stats =
+        at::empty({2, rows_of(x)}, x.options().dtype(at::kFloat));
+    auto [y, h] = run_norm(n, stats);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({want_h ? xr.t : Tensor(),
-                            branch.defined() ? br.t : Tensor(), gate, post,
-                            pre, rbranch, ry});
-    ctx->saved_data["scales"] =
-        std::vector<double>{residual_scale, branch_scale};
-    ctx->saved_data["gate"] = std::vector<int64_t>{gmode, group_rows};
-    ctx->saved_data["needs"] = std::vector<int64_t>{
-        gate.defined() && gate.requires_grad(),
-        post.defined() && post.requires_grad(),
-        pre.defined() && pre.requires_grad()};
+    ctx->save_for_backward(
+        {want_h ? x : Tensor(), n.branch, n.gate, n.post, n.pre, stats});
+    ctx->saved_data["scales"] = c10::complex<double>(residual_scale,
+                                                     branch_scale);
+    ctx->saved_data["group_rows"] = group_rows;
+    const auto needs = [](const Tensor& t) {
+      return t.defined() && t.requires_grad();
+    };
+    ctx->saved_data["gate"] = gmode | needs(n.gate) << 4 | needs(n.post) << 5 |
+                              needs(n.pre) << 6;
     variable_list out;
     if (y.defined()) out.push_back(y);
     if (h.defined()) out.push_back(h);
@@ -269,8 +310,8 @@ struct NormFn : torch::autograd::Function<NormFn> {
     variable_list out(11);
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &branch = saved[1], &gate = saved[2],
-                 &post = saved[3], &pre = saved[4], &rbranch = saved[5],
-                 &ry = saved[6];
+                 &post = saved[3], &pre = saved[4];
+    const float* stats = saved[5].data_ptr<float>();
     Tensor dy, dh;
     if (branch.defined()) {
       dy = grads[0];
@@ -285,13 +326,14 @@ struct NormFn : torch::autograd::Function<NormFn> {
     a.rows = rows_of(some);
     a.dim = some.size(-1);
     a.type = elem(some.scalar_type());
-    const auto scales = ctx->saved_data["scales"].toDoubleVector();
-    const auto g = ctx->saved_data["gate"].toIntVector();
-    const auto needs = ctx->saved_data["needs"].toIntVector();
-    a.residual_scale = (float)scales[0];
-    a.branch_scale = (float)scales[1];
-    a.gmode = (Gate)g[0];
-    a.group_rows = g[1];
+    const auto scales = ctx->saved_data["scales"].toComplexDouble();
+    const int64_t flags = ctx->saved_data["gate"].toInt();
+    const bool needs[3] = {(flags >> 4 & 1) != 0, (flags >> 5 & 1) != 0,
+                           (flags >> 6 & 1) != 0};
+    a.residual_scale = (float)scales.real();
+    a.branch_scale = (float)scales.imag();
+    a.gmode = (Gate)(flags & 15);
+    a.group_rows = ctx->saved_data["group_rows"].toInt();
     Rows xr, br, dyr, dhr;
     Tensor dx = at::empty(some.sizes(), some.options());
     a.dx = dx.data_ptr();
@@ -308,7 +350,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
       a.xstride = xr.stride;
       a.dh = dhr.t.data_ptr();
       a.dhstride = dhr.stride;
-      a.ry = ry.data_ptr<float>();
+      a.ry = stats + a.rows;
       if (pre.defined()) {
         a.pre = pre.data_ptr();
         a.pre32 = pre.scalar_type() == at::kFloat;
@@ -335,7 +377,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
       if (post.defined()) {
         a.post = post.data_ptr();
         a.post32 = post.scalar_type() == at::kFloat;
-        a.rbranch = rbranch.data_ptr<float>();
+        a.rbranch = stats;
         if (needs[1]) {
           dpost = at::empty(post.sizes(), post.options());
           a.dpost = dpost.data_ptr();
@@ -389,9 +431,13 @@ Tensor rms_norm(const Tensor& x, const OptTensor& weight, double eps) {
   TORCH_CHECK(eps >= 0, op, ": eps must not be negative");
   check_device(x, x, op, "x");
   if (weight) check_device(*weight, x, op, "weight");
-  return NormFn::apply(x, OptTensor(), OptTensor(), OptTensor(),
-                       contiguous(weight), 1.0, 1.0, eps, (int64_t)Gate::kNone,
-                       int64_t(1), true)[0];
+  const OptTensor w = contiguous(weight);
+  if (!wants_grad({&x, get(w)}))
+    return std::get<1>(run_norm({x, {}, {}, {}, or_undefined(w), 1.0, 1.0, eps,
+                                 Gate::kNone, 1, true},
+                                Tensor()));
+  return NormFn::apply(x, OptTensor(), OptTensor(), OptTensor(), w, 1.0, 1.0,
+                       eps, (int64_t)Gate::kNone, int64_t(1), true)[0];
 }
 
 std::tuple<Tensor, OptTensor> gated_residual_norm(
@@ -454,11 +500,19 @@ std::tuple<Tensor, OptTensor> gated_residual_norm(
   if (gate) check_device(*gate, x, op, "gate");
   if (post_weight) check_device(*post_weight, x, op, "post_weight");
   if (pre_weight) check_device(*pre_weight, x, op, "pre_weight");
-  auto out = NormFn::apply(x, branch, g, contiguous(post_weight),
-                           contiguous(pre_weight), residual_scale,
+  const OptTensor post = contiguous(post_weight), pre = contiguous(pre_weight);
+  const bool want_h = pre.has_value();
+  if (!wants_grad({&x, &branch, get(g), get(post), get(pre)})) {
+    auto [y, h] = run_norm({x, branch, or_undefined(g), or_undefined(post),
+                            or_undefined(pre), residual_scale, branch_scale,
+                            eps, mode, group_rows, want_h},
+                           Tensor());
+    return {y, want_h ? OptTensor(h) : OptTensor()};
+  }
+  auto out = NormFn::apply(x, branch, g, post, pre, residual_scale,
                            branch_scale, eps, (int64_t)mode, group_rows,
-                           pre_weight.has_value());
-  return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
+                           want_h);
+  return {out[0], want_h ? OptTensor(out[1]) : OptTensor()};
 }
 
 // ---------------------------------------------------------------------------
@@ -516,6 +570,11 @@ void check_codes(const Tensor& codes, const Tensor& exps, int64_t rows,
                   exps.size(1) == pitch / kAct8Group && exps.is_contiguous(),
               op, ": exponents must be contiguous [", rows, ", ",
               pitch / kAct8Group, "], not ", exps.sizes());
+}
+
+void check_wgrad_size(int64_t n, int64_t k, const char* op) {
+  TORCH_CHECK(n <= kAct8MaxCols - kAct8Group && k <= kAct8MaxCols - kAct8Group, op,
+              ": at most ", kAct8MaxCols - kAct8Group, " columns");
 }
 
 void check_codes_aligned(const Tensor& codes, const char* op) {
@@ -593,6 +652,7 @@ std::tuple<Tensor, OptTensor> act8_wgrad_op(const Tensor& dy,
     TORCH_CHECK(dy.size(d) == shape[d], op, ": dy ", dy.sizes(),
                 " does not have the rows of the kept input ",
                 at::IntArrayRef(shape));
+  check_wgrad_size(dy.size(-1), shape.back(), op);
   check_codes(codes, exps, rows_of(dy), shape.back(), op);
   check_device(dy, dy, op, "dy");
   check_device(codes, dy, op, "codes");
@@ -609,7 +669,6 @@ std::tuple<Tensor, OptTensor> act8_wgrad_op(const Tensor& dy,
 struct LinearAct8Fn : torch::autograd::Function<LinearAct8Fn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x,
                         const Tensor& weight, const OptTensor& bias) {
-    const c10::OptionalDeviceGuard guard(x.device());
     Tensor codes, exps;
     const bool grad_b = bias && bias->requires_grad();
     if (weight.requires_grad()) std::tie(codes, exps) = pack_rows(x);
@@ -623,6 +682,8 @@ struct LinearAct8Fn : torch::autograd::Function<LinearAct8Fn> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     no_double_backward("linear_act8");
+    const c10::impl::ExcludeDispatchKeyGuard own_types(
+        c10::autocast_dispatch_keyset);
     const auto saved = ctx->get_saved_variables();
     const auto needs = ctx->saved_data["needs"].toIntVector();
     const Tensor& dy = grads[0];
@@ -650,6 +711,7 @@ Tensor linear_act8(const Tensor& x, const Tensor& weight,
   TORCH_CHECK(weight.dim() == 2 && weight.size(1) == x.size(-1), op,
               ": weight must be [out, ", x.size(-1), "], not ",
               weight.sizes());
+  check_wgrad_size(weight.size(0), weight.size(1), op);
   if (bias) {
     check_act(*bias, op, "bias");
     TORCH_CHECK(bias->scalar_type() == x.scalar_type(), op,
@@ -661,34 +723,48 @@ Tensor linear_act8(const Tensor& x, const Tensor& weight,
   check_device(x, x, op, "x");
   check_device(weight, x, op, "weight");
   if (bias) check_device(*bias, x, op, "bias");
+  // the products are in the arguments' type, under autocast too: the codes
+  // and the gradients go with it
+  const c10::impl::ExcludeDispatchKeyGuard own_types(
+      c10::autocast_dispatch_keyset);
+  const c10::OptionalDeviceGuard guard(x.device());
+  if (!wants_grad({&x, &weight, get(bias)}))
+    return at::linear(x, weight, bias);
   return LinearAct8Fn::apply(x, weight, bias);
+}
+
+// silu(a) * b, and the copies of a and b where they are defined.
+Tensor run_silu(const Tensor& x, const Tensor& codes, const Tensor& exps) {
+  const c10::OptionalDeviceGuard guard(x.device());
+  const Rows xr = as_rows(x);
+  SiluAct8 p = {};
+  p.rows = rows_of(x);
+  p.cols = x.size(-1) / 2;
+  p.pitch = pitch_of(p.cols);
+  p.x = xr.t.data_ptr();
+  p.xstride = xr.stride;
+  p.type = elem(x.scalar_type());
+  c10::SmallVector<int64_t, 6> sizes(x.sizes().begin(), x.sizes().end());
+  sizes.back() = p.cols;
+  Tensor out = at::empty(sizes, x.options());
+  p.out = out.data_ptr();
+  if (codes.defined()) {
+    p.codes = codes.data_ptr<uint8_t>();
+    p.exps = exps.data_ptr<uint8_t>();
+  }
+  check_launch(silu_act8_forward(p, stream_of(x)), "silu_mul_act8");
+  return out;
 }
 
 struct SiluAct8Fn : torch::autograd::Function<SiluAct8Fn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x) {
     const c10::OptionalDeviceGuard guard(x.device());
-    const Rows xr = as_rows(x);
-    SiluAct8 p = {};
-    p.rows = rows_of(x);
-    p.cols = x.size(-1) / 2;
-    p.pitch = pitch_of(p.cols);
-    p.x = xr.t.data_ptr();
-    p.xstride = xr.stride;
-    p.type = elem(x.scalar_type());
-    auto sizes = x.sizes().vec();
-    sizes.back() = p.cols;
-    Tensor out = at::empty(sizes, x.options()), codes, exps;
-    p.out = out.data_ptr();
-    if (x.requires_grad()) {
-      const auto bytes = x.options().dtype(at::kByte);
-      codes = at::empty({p.rows, 2 * p.pitch}, bytes);
-      exps = at::empty({p.rows, 2 * p.pitch / kAct8Group}, bytes);
-      p.codes = codes.data_ptr<uint8_t>();
-      p.exps = exps.data_ptr<uint8_t>();
-    }
-    check_launch(silu_act8_forward(p, stream_of(x)), "silu_mul_act8");
+    const int64_t rows = rows_of(x), pitch = pitch_of(x.size(-1) / 2);
+    const auto bytes = x.options().dtype(at::kByte);
+    const Tensor codes = at::empty({rows, 2 * pitch}, bytes);
+    const Tensor exps = at::empty({rows, 2 * pitch / kAct8Group}, bytes);
     ctx->save_for_backward({codes, exps});
-    return out;
+    return run_silu(x, codes, exps);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -722,6 +798,7 @@ Tensor silu_mul_act8(const Tensor& x) {
               ": x must hold two halves in its last dimension, not ",
               x.size(-1), " columns");
   check_device(x, x, op, "x");
+  if (!wants_grad({&x})) return run_silu(x, Tensor(), Tensor());
   return SiluAct8Fn::apply(x);
 }
 

@@ -215,6 +215,25 @@ def test_linear_act8():
         assert torch.equal(torch.autograd.grad(y, x, dy)[0], dx)
 
 
+def test_linear_act8_of_one_row_and_under_autocast():
+    from baguanet import ops
+
+    x = rows((96,), F32).cuda().requires_grad_()
+    w = rows((50, 96), F32, 1, wild=False).cuda().requires_grad_()
+    b = rows((50,), F32, 2, wild=False).cuda().requires_grad_()
+    dy = rows((50,), F32, 3, wild=False).cuda()
+    want = torch.autograd.grad(ops.linear_act8(x, w, b), (x, w, b), dy)
+    assert want[1].equal(torch.outer(dy, ops.act8_unpack(ops.act8_pack(x))))
+    with torch.autocast("cuda", torch.bfloat16):
+        y = ops.linear_act8(x, w, b)
+        got = torch.autograd.grad(y, (x, w, b), dy)
+    assert y.dtype == F32  # it computes in its arguments' type
+    assert all(torch.equal(g, v) for g, v in zip(got, want))
+    with torch.no_grad():
+        assert torch.equal(ops.linear_act8(x, w, b),
+                           torch.nn.functional.linear(x, w, b))
+
+
 def test_linear_act8_holds_codes_only():
     from baguanet import ops
 

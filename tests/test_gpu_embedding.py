@@ -118,6 +118,22 @@ def test_only_padding():
     assert (dw == 0).all()
 
 
+def test_one_token_without_dimensions():
+    from baguanet import ops
+
+    w = torch.randn(9, 40, device="cuda", requires_grad=True)
+    tok = torch.tensor(4, device="cuda")
+    y = ops.embedding(w, tok, scale=2.0)
+    assert y.shape == (40,) and torch.equal(y, 2.0 * w[4])
+    (dw,) = torch.autograd.grad(y.sum(), w)
+    want = torch.zeros_like(w)
+    want[4] = 2.0
+    assert torch.equal(dw, want)
+    with torch.no_grad():
+        out = ops.embedding(w, tok[None], scale=2.0)
+    assert torch.equal(out[0], y) and not out.requires_grad
+
+
 def test_no_tokens():
     from baguanet import ops
 

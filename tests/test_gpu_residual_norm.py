@@ -126,7 +126,7 @@ def case(shape, dtype=BF, gate=None, post=True, pre=True, wtype=F32,
         check(got[k], *v, what=k)
 
 
-@pytest.mark.parametrize("dim", [1, 2, 7, 64, 511, 512, 513, 1000, 1024, 1025,
+@pytest.mark.parametrize("dim", [1, 2, 7, 8, 9, 15, 64, 511, 512, 513, 1000, 1024, 1025,
                                  2048, 2049, 4096, 4100, 8192, 8193, 12289,
                                  16383, 16384])
 def test_widths(dim):
@@ -206,6 +206,24 @@ def test_rms_norm():
             check(grads[0], *ref["dx"], what="dx")
             if weight:
                 check(grads[1], *ref["dpre"], what="dw")
+
+
+def test_one_row_and_no_grad():
+    from baguanet import ops
+
+    x, o = (torch.randn(600, device="cuda", requires_grad=True)
+            for _ in range(2))
+    w = torch.rand(600, device="cuda", requires_grad=True)
+    y, h = ops.gated_residual_norm(x, o, w, w, w, branch_scale=0.5)
+    assert y.requires_grad and h.requires_grad
+    with torch.no_grad():
+        y1, h1 = ops.gated_residual_norm(x, o, w, w, w, branch_scale=0.5)
+        assert torch.equal(y, y1) and torch.equal(h, h1)
+        y1, h1 = ops.gated_residual_norm(x[None], o[None], w, w, None, 1, 0.5)
+        assert h1 is None and torch.equal(y, y1[0])
+        n1 = ops.rms_norm(x, w)
+    assert not n1.requires_grad
+    assert torch.equal(ops.rms_norm(x, w), n1)
 
 
 def test_empty():
