@@ -1,0 +1,236 @@
+"""The training-step operators together, as a language model's step uses them:
+embedding, gated residual norms between blocks, blocks whose activations are
+kept in 8 bits, under BucketedDDP and FusedSGD."""
+
+import pytest
+import torch
+from torch import nn
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+U = 2.0 ** -24
+
+
+class Block(nn.Module):
+    def __init__(self, dim, hidden, dtype):
+        super().__init__()
+        rand = lambda *s: nn.Parameter((torch.randn(*s) * s[-1] ** -0.5)
+                                       .to(dtype))
+        self.up, self.down = rand(2 * hidden, dim), rand(dim, hidden)
+        self.bias = nn.Parameter(torch.zeros(2 * hidden, dtype=dtype))
+        self.gate = nn.Parameter(torch.ones(dim) * 0.5)
+        self.post = nn.Parameter(torch.ones(dim))
+        self.pre = nn.Parameter(torch.ones(dim))
+
+    def forward(self, x, h):
+        from baguanet import ops
+
+        up = ops.linear_act8(h, self.up, self.bias)
+        down = ops.linear_act8(ops.silu_mul_act8(up), self.down)
+        return ops.gated_residual_norm(x, down, self.gate, self.post,
+                                       self.pre, branch_scale=0.7)
+
+
+class Net(nn.Module):
+    def __init__(self, vocab=97, dim=136, hidden=200, blocks=3, dtype=BF):
+        super().__init__()
+        torch.manual_seed(0)
+        self.table = nn.Parameter((torch.randn(vocab, dim) * 0.1).to(dtype))
+        self.first = nn.Parameter(torch.ones(dim))
+        self.blocks = nn.ModuleList(Block(dim, hidden, dtype)
+                                    for _ in range(blocks))
+        self.kept = {}
+
+    def forward(self, tokens):
+        from baguanet import ops
+
+        x = ops.embedding(self.table, tokens, scale=dim_scale(self.table),
+                          padding_idx=0)
+        self.kept["x"] = x
+        h = ops.rms_norm(x, self.first)
+        for b in self.blocks:
+            x, h = b(x, h)
+        self.kept["h"] = h
+        logits = ops.linear_act8(h, self.table)  # the table is shared
+        self.kept["logits"] = logits
+        return logits
+
+
+def dim_scale(table):
+    return float(table.shape[1]) ** 0.5
+
+
+def _batch(seed, n=(4, 33)):
+    g = torch.Generator().manual_seed(seed)
+    tok = torch.randint(0, 97, n, generator=g)
+    tok[:, -3:] = 0  # padding
+    return tok.cuda(), torch.randint(0, 97, n, generator=g).cuda()
+
+
+def _loss(model, batch):
+    logits = model(batch[0]).float()
+    return nn.functional.cross_entropy(logits.flatten(0, -2),
+                                       batch[1].flatten())
+
+
+def _grads(batches, dtype=BF):
+    model = Net(dtype=dtype).cuda()
+    out = []
+    for b in batches:
+        params = list(model.parameters())
+        out.append(torch.autograd.grad(_loss(model, b), params))
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_same_gradients_in_buckets(dtype):
+    from baguanet.parallel import BucketedDDP
+
+    batches = [_batch(1), _batch(2)]
+    want = _grads(batches, dtype)
+    model = BucketedDDP(Net(dtype=dtype).cuda(), bucket_cap_mb=0.1,
+                        broadcast_params=False)
+    assert len(model.buckets) > 1
+    model.zero_grad()
+    _loss(model, batches[0]).backward()
+    model.finish_backward()
+    params = list(model.module.parameters())
+    for p, g in zip(params, want[0]):
+        assert torch.equal(p.grad, g)
+    # a second micro-batch adds up in the buckets
+    _loss(model, batches[1]).backward()
+    model.finish_backward()
+    for p, a, b in zip(params, *want):
+        # one of the two sums of the shared table's parts may come first
+        both = a.double() + b.double()
+        tol = torch.finfo(p.dtype).eps * (a.abs().double() + b.abs().double())
+        assert ((p.grad.double() - both).abs() <= tol + 1e-30).all()
+
+
+def test_steps_with_fused_sgd():
+    """Three steps of the optimizer are those of its rule on the gradients,
+    and the same in a second run."""
+    from baguanet.optim import FusedSGD
+    from baguanet.parallel import BucketedDDP
+
+    def train():
+        model = BucketedDDP(Net(dtype=torch.float32).cuda(),
+                            broadcast_params=False)
+        opt = FusedSGD(model.parameters(), lr=0.05, momentum=0.9)
+        params = list(model.module.parameters())
+        mom = [torch.zeros_like(p) for p in params]
+        for i in range(3):
+            model.zero_grad()
+            loss = _loss(model, _batch(i))
+            loss.backward()
+            model.finish_backward()
+            assert torch.isfinite(loss)
+            before = [p.detach().clone() for p in params]
+            opt.step()
+            for p, old, m in zip(params, before, mom):
+                m.mul_(0.9).add_(p.grad)
+                # two fp32 products and sums, in one order or another
+                tol = 4 * U * (old.abs() + 0.05 * 2 * m.abs())
+                tol = tol + 4 * U * 0.05 * p.grad.abs()
+                assert ((p - (old - 0.05 * m)).abs() <= tol).all()
+        return params
+
+    for a, b in zip(train(), train()):
+        assert torch.equal(a, b)
+
+
+def test_table_gradient_of_both_uses():
+    """The shared table's gradient, from what passed through both operators
+    that use it, in 64 bits."""
+    from baguanet import ops
+
+    model = Net(dtype=torch.float32).cuda()
+    batch = _batch(5)
+    loss = _loss(model, batch)
+    for t in model.kept.values():
+        t.retain_grad()
+    loss.backward()
+    x, h, logits = (model.kept[k] for k in ("x", "h", "logits"))
+    dy = logits.grad.double().flatten(0, -2)
+    kept = ops.act8_unpack(ops.act8_pack(h.detach())).double().flatten(0, -2)
+    head, head_mag = dy.t() @ kept, dy.abs().t() @ kept.abs()
+    tok = batch[0].flatten()
+    live = tok != 0
+    dx = x.grad.double().flatten(0, -2)[live]
+    look = torch.zeros_like(head).index_add_(0, tok[live], dx)
+    look_mag = torch.zeros_like(head).index_add_(0, tok[live], dx.abs())
+    s = dim_scale(model.table)
+    want = head + s * look
+    # fp32 sums over 132 rows, three times as many in the product of a
+    # gradient split in three, one step of 2**-23 each at most
+    tol = (3 * 132 + 8) * 2 * U * (head_mag + s * look_mag) + 2 * U * want.abs()
+    assert ((model.table.grad.double() - want).abs() <= tol).all()
+
+
+def test_holds_less_memory():
+    """What a block's forward pass leaves for the backward pass."""
+    from baguanet import ops
+
+    torch.manual_seed(0)
+    rows, dim, hidden = 4096, 1024, 2048
+    block = Block(dim, hidden, BF).cuda()
+    x = torch.randn(rows, dim, device="cuda").to(BF).requires_grad_()
+    h = torch.randn(rows, dim, device="cuda").to(BF).requires_grad_()
+
+    def held(f):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        out = f()
+        now = torch.cuda.memory_allocated() - before
+        del out
+        return now
+
+    def plain():
+        up = nn.functional.linear(h, block.up, block.bias)
+        a, b = up.chunk(2, -1)
+        down = nn.functional.linear(nn.functional.silu(a) * b, block.down)
+        return ops.gated_residual_norm(x, down, block.gate, block.post,
+                                       block.pre, branch_scale=0.7)
+
+    ours, theirs = held(lambda: block(x, h)), held(plain)
+    # outputs y and h and the branch: 6 bytes a column; codes of the two
+    # linear inputs and the gated activation's two: 33/32 of a byte each
+    most = rows * (6 * dim + 33 / 32 * (dim + hidden + 2 * hidden))
+    assert ours <= most + 16 * 2 ** 21
+    # plain: silu's input and result, both factors, the product: 2 bytes each
+    assert theirs - ours >= rows * hidden * 2
+
+
+def test_whole_step_in_a_graph():
+    """Forward and backward of the whole net, captured and replayed."""
+    model = Net(dtype=torch.float32).cuda()
+    params = list(model.parameters())
+    batch = _batch(1)
+
+    def step():
+        logits = model(batch[0])
+        return torch.autograd.grad(logits, params, torch.ones_like(logits))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    model.kept.clear()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    model.kept.clear()
+    for i in range(4):
+        for t, s in zip(batch, _batch(10 + i)):
+            t.copy_(s)
+        with torch.no_grad():
+            for p in params:
+                p.mul_(0.9)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        model.kept.clear()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
