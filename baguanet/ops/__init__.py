@@ -7,6 +7,7 @@ extension raises — the HIP path must never silently fall back to eager.
 
 from __future__ import annotations
 
+import importlib.util
 import os
 from pathlib import Path
 from typing import NamedTuple
@@ -19,42 +20,69 @@ _C = None
 _ERR: Exception | None = None
 
 
-def build_extension(verbose: bool = False):
-    """Compile (if needed) and load the extension; in-tree build dir."""
-    global _C, _ERR
-    if _C is not None:
-        return _C
-    from torch.utils import cpp_extension
-
-    os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
-    build_dir = REPO_ROOT / "build" / "torch_ext"
-    build_dir.mkdir(parents=True, exist_ok=True)
+def _sources() -> list[Path]:
     src = REPO_ROOT / "csrc"
+    return [
+        src / "torch" / "ops.cc",
+        src / "torch" / "train_ops.cc",
+        src / "hip" / "pack_kernels.hip",
+        src / "hip" / "multi_tensor.hip",
+        src / "hip" / "embedding.hip",
+        src / "hip" / "residual_norm.hip",
+        src / "hip" / "act8.hip",
+        src / "hip" / "act8_wgrad.hip",
+    ]
+
+
+def _import_built(lib: Path):
+    spec = importlib.util.spec_from_file_location("baguanet_C", lib)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def build_extension(verbose: bool = False, force: bool = False):
+    """Load the extension from its in-tree build dir, compiled first if it is
+    missing or older than its sources, or always with ``force``."""
+    global _C, _ERR
+    if _C is not None and not force:
+        return _C
+    build_dir = REPO_ROOT / "build" / "torch_ext"
+    lib = build_dir / "baguanet_C.so"
     try:
-        _C = cpp_extension.load(
-            name="baguanet_C",
-            sources=[
-                str(src / "torch" / "ops.cc"),
-                str(src / "torch" / "train_ops.cc"),
-                str(src / "hip" / "pack_kernels.hip"),
-                str(src / "hip" / "multi_tensor.hip"),
-                str(src / "hip" / "embedding.hip"),
-                str(src / "hip" / "residual_norm.hip"),
-                str(src / "hip" / "act8.hip"),
-                str(src / "hip" / "act8_wgrad.hip"),
-            ],
-            build_directory=str(build_dir),
-            extra_cflags=["-O3"],
-            # packed fp32 instructions stay out of every kernel: some of
-            # their forms have given wrong results on this hardware
-            extra_cuda_cflags=["-O3", "-Xclang", "-target-feature",
-                               "-Xclang", "-packed-fp32-ops"],
-            verbose=verbose,
-        )
+        sources = _sources()
+        headers = list((REPO_ROOT / "csrc" / "hip").glob("*.h"))
+        newest = max(p.stat().st_mtime for p in sources + headers)
+        if force or not lib.exists() or lib.stat().st_mtime < newest:
+            _C = _compile(build_dir, sources, verbose, force)
+        else:
+            _C = _import_built(lib)
     except Exception as e:  # pragma: no cover
         _ERR = e
         raise
     return _C
+
+
+def _compile(build_dir: Path, sources: list[Path], verbose: bool,
+             force: bool):
+    from torch.utils import cpp_extension
+
+    os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
+    build_dir.mkdir(parents=True, exist_ok=True)
+    if force:
+        for built in build_dir.glob("*.o"):
+            built.unlink()
+    return cpp_extension.load(
+        name="baguanet_C",
+        sources=[str(p) for p in sources],
+        build_directory=str(build_dir),
+        extra_cflags=["-O3"],
+        # packed fp32 instructions stay out of every kernel: some of their
+        # forms have given wrong results on this hardware
+        extra_cuda_cflags=["-O3", "-Xclang", "-target-feature", "-Xclang",
+                           "-packed-fp32-ops"],
+        verbose=verbose,
+    )
 
 
 def _load():
