@@ -29,9 +29,9 @@
 namespace baguanet {
 namespace {
 
-// Sums of N values over the TPR threads of a row.  `red` is one of two
-// buffers used in turn, which saves the second barrier: a buffer is written
-// again only after the barrier of the other.
+// Sums of N values over the TPR threads of a row.  `red` must be each of two
+// buffers in turn, from call to call, which saves the second barrier: a buffer
+// is written again only after the barrier of the other.
 template <int TPR, int N>
 __device__ inline void row_sums(float (&v)[N], float* red) {
 #pragma unroll
@@ -96,6 +96,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_forward_kernel(
     }
   };
   if (row < a.rows) fetch(row);
+  int parity = 0;
   for (; row < a.rows; row += step) {
     float8 y[VPT], o[VPT];
 #pragma unroll
@@ -110,7 +111,8 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_forward_kernel(
         float s[1] = {0.f};
 #pragma unroll
         for (int j = 0; j < VPT; j++) s[0] += c[j].sum(o[j] * o[j]);
-        row_sums<TPR>(s, red[0]);
+        row_sums<TPR>(s, red[parity]);
+        parity ^= 1;
         ro = 1.f / sqrtf(s[0] * inv_dim + a.eps);
         if (lane == 0 && a.rbranch) a.rbranch[row] = ro;
       }
@@ -134,7 +136,8 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_forward_kernel(
       float s[1] = {0.f};
 #pragma unroll
       for (int j = 0; j < VPT; j++) s[0] += c[j].sum(y[j] * y[j]);
-      row_sums<TPR>(s, red[1]);
+      row_sums<TPR>(s, red[parity]);
+      parity ^= 1;
       const float ry = 1.f / sqrtf(s[0] * inv_dim + a.eps);
       if (lane == 0 && a.ry) a.ry[row] = ry;
 #pragma unroll
@@ -531,7 +534,8 @@ hipError_t norm_forward(const NormFwd& a, hipStream_t stream) {
       const int64_t teams = kBlk / kTpr;
       const int64_t want = (a.rows + teams - 1) / teams;
       const int64_t most = 256 * 2048 / kBlk;
-      launch(norm_forward_kernel<T, kTpr, kVpt, kTiny>, (uint32_t)(want < most ? want : most), kBlk, stream, a);
+      launch(norm_forward_kernel<T, kTpr, kVpt, kTiny>,
+             (uint32_t)(want < most ? want : most), kBlk, stream, a);
     });
   });
   return hipGetLastError();
@@ -563,16 +567,17 @@ hipError_t norm_backward(const NormBwd& a, hipStream_t stream) {
       const bool seam = a.branch && a.post && a.dy && a.dh &&
                         (a.gmode == Gate::kNone || a.gmode == Gate::kGroup);
       if (seam)
-        launch(norm_backward_kernel<T, kTpr, kVpt, kTiny, true>, (uint32_t)c.blocks,
-               block_of<kTpr>(), stream, a, c, parts);
+        launch(norm_backward_kernel<T, kTpr, kVpt, kTiny, true>,
+               (uint32_t)c.blocks, block_of<kTpr>(), stream, a, c, parts);
       else
-        launch(norm_backward_kernel<T, kTpr, kVpt, kTiny, false>, (uint32_t)c.blocks,
-               block_of<kTpr>(), stream, a, c, parts);
+        launch(norm_backward_kernel<T, kTpr, kVpt, kTiny, false>,
+               (uint32_t)c.blocks, block_of<kTpr>(), stream, a, c, parts);
     });
     if (parts.pre || parts.post || parts.group) {
       const dim3 grid((uint32_t)((a.dim + kJoinCols - 1) / kJoinCols),
                       (uint32_t)(2 + (parts.group ? c.groups : 0)));
-      launch(norm_join_kernel<T>, grid, kJoinCols * kJoinStrips, stream, a, c, parts);
+      launch(norm_join_kernel<T>, grid, kJoinCols * kJoinStrips, stream, a, c,
+             parts);
     }
   });
   return hipGetLastError();

@@ -622,7 +622,8 @@ std::tuple<Tensor, Tensor> wgrad_rows(const Tensor& dy, const Tensor& codes,
   Tensor dw = at::empty({a.n, a.k}, dy.options());
   Tensor db = bias ? at::empty({a.n}, dy.options()) : Tensor();
   if (a.m == 0) dw.zero_();
-  if (bias && (a.m == 0 || a.k == 0)) db.copy_(dy.reshape({-1, a.n}).sum(0));
+  if (bias && (a.m == 0 || a.k == 0))
+    db.copy_(dy.reshape({a.m, a.n}).sum(0));
   a.dy = dr.t.data_ptr();
   a.dstride = dr.stride;
   a.codes = codes.data_ptr<uint8_t>();
@@ -663,6 +664,17 @@ std::tuple<Tensor, OptTensor> act8_wgrad_op(const Tensor& dy,
   return {dw, bias ? OptTensor(db) : OptTensor()};
 }
 
+// One product of matrices whatever x's layout: as batches of small ones with
+// a transposed operand, which the library makes of some layouts, it has
+// faulted on this hardware.
+Tensor flat_linear(const Tensor& x, const Tensor& weight,
+                   const OptTensor& bias) {
+  auto sizes = x.sizes().vec();
+  sizes.back() = weight.size(0);
+  return at::linear(x.reshape({rows_of(x), x.size(-1)}), weight, bias)
+      .view(sizes);
+}
+
 // A linear layer whose input is kept in 8 bits.  Its two plain products, y
 // and dx, are the library's, as in torch.nn.Linear; the weight gradient is
 // taken from the codes.
@@ -677,7 +689,7 @@ struct LinearAct8Fn : torch::autograd::Function<LinearAct8Fn> {
     ctx->saved_data["needs"] = std::vector<int64_t>{
         x.requires_grad(), weight.requires_grad(), grad_b};
     ctx->saved_data["k"] = x.size(-1);
-    return at::linear(x, weight, bias);
+    return flat_linear(x, weight, bias);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -689,13 +701,18 @@ struct LinearAct8Fn : torch::autograd::Function<LinearAct8Fn> {
     const Tensor& dy = grads[0];
     const c10::OptionalDeviceGuard guard(dy.device());
     variable_list out(3);
-    if (needs[0]) out[0] = at::matmul(dy, saved[0]);
+    if (needs[0]) {
+      auto sizes = dy.sizes().vec();
+      sizes.back() = saved[0].size(1);
+      out[0] = at::mm(dy.reshape({rows_of(dy), dy.size(-1)}), saved[0])
+                   .view(sizes);
+    }
     if (needs[1])
       std::tie(out[1], out[2]) =
           wgrad_rows(dy, saved[1], saved[2], ctx->saved_data["k"].toInt(),
                      needs[2]);
     else if (needs[2])
-      out[2] = dy.reshape({-1, dy.size(-1)}).sum(0);
+      out[2] = dy.reshape({rows_of(dy), dy.size(-1)}).sum(0);
     return out;
   }
 };
@@ -729,7 +746,7 @@ Tensor linear_act8(const Tensor& x, const Tensor& weight,
       c10::autocast_dispatch_keyset);
   const c10::OptionalDeviceGuard guard(x.device());
   if (!wants_grad({&x, &weight, get(bias)}))
-    return at::linear(x, weight, bias);
+    return flat_linear(x, weight, bias);
   return LinearAct8Fn::apply(x, weight, bias);
 }
 

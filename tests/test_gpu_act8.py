@@ -215,6 +215,28 @@ def test_linear_act8():
         assert torch.equal(torch.autograd.grad(y, x, dy)[0], dx)
 
 
+def test_linear_act8_layouts():
+    """Inputs and gradients that do not collapse to rows."""
+    from baguanet import ops
+
+    big = rows((6, 20, 130), BF).cuda()
+    w = rows((48, 64), BF, 1, wild=False).cuda().requires_grad_()
+    for x in (big[..., 3:67], big[:, :, :64].transpose(0, 1),
+              big[:, ::3, 5:69], big[:1, :1, :64].expand(5, 7, 64)):
+        a, b = (v.detach().requires_grad_() for v in (x, x.contiguous()))
+        ya, yb = ops.linear_act8(a, w), ops.linear_act8(b, w)
+        assert torch.equal(ya, yb)
+        d = rows((*x.shape[:-1], 48), BF, 2, wild=False).cuda()
+        for g in (d, d.transpose(0, 1).contiguous().transpose(0, 1),
+                  d[..., :1].expand_as(d), d[:, :1].expand_as(d)):
+            ga = torch.autograd.grad(ya, (a, w), g, retain_graph=True)
+            gb = torch.autograd.grad(yb, (b, w), g.contiguous(),
+                                     retain_graph=True)
+            assert all(torch.equal(p, q) for p, q in zip(ga, gb))
+        with torch.no_grad():
+            assert torch.equal(ops.linear_act8(x, w), ya)
+
+
 def test_linear_act8_of_one_row_and_under_autocast():
     from baguanet import ops
 

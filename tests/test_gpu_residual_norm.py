@@ -208,6 +208,29 @@ def test_rms_norm():
                 check(grads[1], *ref["dpre"], what="dw")
 
 
+@pytest.mark.parametrize("dim", [600, 2000, 4096, 8000, 16384])
+def test_each_row_is_its_own(dim):
+    """With many rows for each workgroup, every row comes out as it does in a
+    call of its own few: sums over rows of one workgroup do not meet."""
+    from baguanet import ops
+
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    rows = 6000 if dim > 8192 else 12000
+    x = torch.randn(rows, dim, device="cuda", generator=g)
+    x *= torch.rand(rows, 1, device="cuda", generator=g) * 100
+    w = torch.rand(dim, device="cuda", generator=g)
+    o = x.flip(0)
+    calls = [lambda a, b: ops.rms_norm(a, w),
+             lambda a, b: ops.gated_residual_norm(a, b, w, None, w)[1],
+             lambda a, b: ops.gated_residual_norm(a, b, w, w, None)[0],
+             lambda a, b: ops.gated_residual_norm(a, b, w, w, w)[1]]
+    for call in calls:
+        whole = call(x, o)
+        for i in range(0, rows, 250):
+            s = slice(i, i + 250)
+            assert torch.equal(whole[s], call(x[s], o[s]))
+
+
 def test_one_row_and_no_grad():
     from baguanet import ops
 
