@@ -609,6 +609,8 @@ Tensor act8_unpack_op(const Tensor& codes, const Tensor& exps,
   return x;
 }
 
+Tensor bias_rows(const Tensor& dy);
+
 std::tuple<Tensor, Tensor> wgrad_rows(const Tensor& dy, const Tensor& codes,
                                       const Tensor& exps, int64_t k,
                                       bool bias) {
@@ -621,9 +623,12 @@ std::tuple<Tensor, Tensor> wgrad_rows(const Tensor& dy, const Tensor& codes,
   a.pitch = pitch_of(k);
   Tensor dw = at::empty({a.n, a.k}, dy.options());
   Tensor db = bias ? at::empty({a.n}, dy.options()) : Tensor();
-  if (a.m == 0) dw.zero_();
-  if (bias && (a.m == 0 || a.k == 0))
-    db.copy_(dy.reshape({a.m, a.n}).sum(0));
+  if (a.m == 0) {
+    dw.zero_();
+    if (bias) db.zero_();
+  } else if (bias && a.k == 0) {
+    db = bias_rows(dy);
+  }
   a.dy = dr.t.data_ptr();
   a.dstride = dr.stride;
   a.codes = codes.data_ptr<uint8_t>();
@@ -635,6 +640,16 @@ std::tuple<Tensor, Tensor> wgrad_rows(const Tensor& dy, const Tensor& codes,
   a.workspace = ws.data_ptr();
   check_launch(act8_wgrad(a, stream_of(dy)), "act8_wgrad");
   return {dw, db};
+}
+
+// The sum of dy's rows alone, beside a product with one column of zeros.
+// (torch's sum clears memory in a way that a captured graph does not repeat
+// reliably on this hardware.)
+Tensor bias_rows(const Tensor& dy) {
+  const auto bytes = dy.options().dtype(at::kByte);
+  const int64_t rows = rows_of(dy);
+  return std::get<1>(wgrad_rows(dy, at::zeros({rows, kAct8Group}, bytes),
+                                at::zeros({rows, 1}, bytes), 1, true));
 }
 
 std::tuple<Tensor, OptTensor> act8_wgrad_op(const Tensor& dy,
@@ -712,7 +727,7 @@ struct LinearAct8Fn : torch::autograd::Function<LinearAct8Fn> {
           wgrad_rows(dy, saved[1], saved[2], ctx->saved_data["k"].toInt(),
                      needs[2]);
     else if (needs[2])
-      out[2] = dy.reshape({rows_of(dy), dy.size(-1)}).sum(0);
+      out[2] = bias_rows(dy);
     return out;
   }
 };
