@@ -394,8 +394,9 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(
 // The runs that cross chunk borders, each summed from its parts by one
 // workgroup for a tile of columns: its threads look for the run's end
 // together, each of its teams adds up every so many of the parts, and the
-// teams' sums are added in their order.
-constexpr int kJoinBlock = 1024;
+// teams' sums are added in their order.  Teams have 128 lanes at most, so
+// that the hundreds of parts of the most frequent token are shared by four.
+constexpr int kJoinBlock = 512, kJoinBlocks = 1024;
 
 template <typename W, bool kTiny>
 __global__ __launch_bounds__(kJoinBlock) void embedding_join_kernel(
@@ -403,11 +404,12 @@ __global__ __launch_bounds__(kJoinBlock) void embedding_join_kernel(
   __shared__ int wave_end[kJoinBlock / kWave];
   __shared__ float joint[kJoinBlock * kVec];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const int tpr = ch.tpr, teams = kJoinBlock / tpr;
+  const int tpr = ch.tpr < 128 ? ch.tpr : 128, teams = kJoinBlock / tpr;
   const int team = threadIdx.x / tpr, in = threadIdx.x % tpr;
-  const int64_t items = *starts.count * ch.tiles;
+  const int64_t tiles = (a.dim + tpr * kVec - 1) / (tpr * kVec);
+  const int64_t items = *starts.count * tiles;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int64_t chunk = starts.chunk[item / ch.tiles];
+    const int64_t chunk = starts.chunk[item / tiles];
     const int32_t key = s.key[(chunk + 1) * ch.size - 1];
     // chunks that begin with the key hold a part in slot 0
     int64_t parts = 1;
@@ -424,13 +426,13 @@ __global__ __launch_bounds__(kJoinBlock) void embedding_join_kernel(
       }
       __syncthreads();
     }
-    int64_t at = ((item % ch.tiles) * tpr + in) * kVec;
+    int64_t at = ((item % tiles) * tpr + in) * kVec;
     if (kTiny)
       at = 0;
     else if (at + kVec > a.dim)
       at = a.dim - kVec;
     const Cols<kTiny> c(0, kTiny ? (int)a.dim : kVec);
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;
     float8 acc = 0.f;
     for (int64_t j = team; j < parts; j += teams * kAhead) {
       float8 part[kAhead];
@@ -601,11 +603,8 @@ hipError_t embedding_backward(const EmbeddingBwd& a, hipStream_t stream) {
                stream, a, sorted, ch, starts, partial);
       });
       if (ch.count > 1)
-        launch(embedding_join_kernel<W, kTiny>,
-               (uint32_t)(ch.count * ch.tiles < 512 ? ch.count * ch.tiles
-                                                    : 512),
-               kJoinBlock, stream, a, sorted, ch, starts,
-               (const float*)partial);
+        launch(embedding_join_kernel<W, kTiny>, kJoinBlocks, kJoinBlock, stream,
+               a, sorted, ch, starts, (const float*)partial);
     };
     if (a.dim < kVec)
       sums(std::true_type());
