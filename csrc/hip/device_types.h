@@ -137,7 +137,8 @@ struct Cols {
     }
 #pragma unroll
     for (int i = 0; i < kVec; i++)
-      if (i >= dup && i < count) row[col + i] = first ? v[i] : row[col + i] + v[i];
+      if (i >= dup && i < count)
+        row[col + i] = first ? v[i] : row[col + i] + v[i];
   }
   // The sum of the lane's own columns.
   __device__ inline float sum(float8 v) const {
@@ -148,7 +149,6 @@ struct Cols {
     return sum8(v);
   }
 };
-
 
 // Launches a kernel without dynamic LDS.
 template <typename... P>

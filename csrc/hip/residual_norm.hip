@@ -13,6 +13,8 @@
 //   dg = sum over the gate's elements of bs * post * dY * no
 //
 // Both passes are bound by HBM: 4 row reads and writes forward, 6 backward.
+// 32768 rows of 8192 bf16: forward 378 us (5.7 TB/s), backward 636 (5.1) and 8
+// for the join; backward 3.9 TB/s above 8192 columns.  A large copy moves 5.0.
 // A row stays in its team's registers between the sums over it and their
 // use, the next row's loads are issued before them, and the weights are read
 // once for all rows of a team.  The sums over rows (dpre, dpost, dg) stay in

@@ -573,8 +573,8 @@ void check_codes(const Tensor& codes, const Tensor& exps, int64_t rows,
 }
 
 void check_wgrad_size(int64_t n, int64_t k, const char* op) {
-  TORCH_CHECK(n <= kAct8MaxCols - kAct8Group && k <= kAct8MaxCols - kAct8Group, op,
-              ": at most ", kAct8MaxCols - kAct8Group, " columns");
+  constexpr int64_t most = kAct8MaxCols - kAct8Group;
+  TORCH_CHECK(n <= most && k <= most, op, ": at most ", most, " columns");
 }
 
 void check_codes_aligned(const Tensor& codes, const char* op) {
