@@ -13,7 +13,8 @@ multi-TCP-stream network transport plugin) for AMD MI355X clusters:
 * ``baguanet.models`` — VGG16 / ResNet-50 for the reference's benchmark
   workloads (BASELINE.md).
 * ``baguanet.ops`` — HIP staging/pack kernels exposed to torch for tests
-  and microbenchmarks.
+  and microbenchmarks, and the training-step operators (embedding, gated
+  residual norm, 8-bit activation checkpoints) with their gradients.
 """
 
 __version__ = "0.1.0"
