@@ -38,6 +38,7 @@ typedef fp16 fp16x8 __attribute__((ext_vector_type(8)));
 constexpr int kThreads = 256;  // four waves, two by two
 constexpr int kTM = 64;         // rows summed for each tile in LDS
 constexpr int kSteps = kTM / 16;  // of the matrix instructions for a tile
+constexpr int kUnits = 256;       // compute units
 
 template <typename T>
 __device__ inline float16v mfma(short8v a, short8v b, float16v c);
@@ -110,25 +111,31 @@ __device__ inline __amdgpu_buffer_rsrc_t descriptor(const char* p, int size) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, size, 0x00027000);
 }
 
-// One product: dy in tiles of kTM rows, `tiles` in all; x' starts again
-// after `xtiles` of them (the planes of an fp32 gradient).
+// A part of dW: its rows and columns from the first up to the end.
+struct Part {
+  int64_t n0, n1, k0, k1;
+  int ntiles, ktiles;
+};
+
+// One product, for a part of dW: dy in tiles of kTM rows, `tiles` in all; x'
+// starts again after `xtiles` of them (the planes of an fp32 gradient).
 struct Product {
   Stream dy, codes, exps;
   int dpitch, cpitch;      // bytes between rows of dy and of codes
   int tiles, xtiles;
   int slices, slice_tiles;
-  int ntiles, ktiles;
-  int64_t n, k;
+  Part part;
+  int64_t k;            // columns of dW
   void* dw;
-  void* db;                // null: not wanted
-  float* partial;          // [slices, n, k] where slices > 1
-  float* bias_partial;     // [slices, n] where slices > 1
+  void* db;             // null: not wanted, or not from this part
+  float* partial;       // [slices, rows, columns of the part], slices > 1
+  float* bias_partial;  // [slices, rows of the part], slices > 1
 };
 
 // The workgroup's tile of dW.  Workgroups go to the 8 XCDs in turn; each XCD
 // takes a run of tiles, in strips 8 tiles high, so that those at work
 // together read the same parts of dy and x' through its L2.
-__device__ inline void pick_tile(const Product& p, int& tn, int& tk) {
+__device__ inline void pick_tile(const Part& p, int& tn, int& tk) {
   const int total = p.ntiles * p.ktiles, id = blockIdx.x;
   const int xcd = id % 8, each = total / 8, more = total % 8;
   const int at = xcd * each + (xcd < more ? xcd : more) + id / 8;
@@ -186,8 +193,9 @@ void act8_wgrad_kernel(Product p) {
   constexpr int kTile = kTM * (kTN + kTK);  // both operands' tiles
   __shared__ __attribute__((aligned(16))) short lds[2 * kTile];
   int tn, tk;
-  pick_tile(p, tn, tk);
-  const int64_t n0 = (int64_t)tn * kTN, k0 = (int64_t)tk * kTK;
+  pick_tile(p.part, tn, tk);
+  const int64_t n0 = p.part.n0 + (int64_t)tn * kTN;
+  const int64_t k0 = p.part.k0 + (int64_t)tk * kTK;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int wn = (wave / 2) * (kTN / 2), wk = (wave % 2) * (kTK / 2);
   const int t0 = blockIdx.y * p.slice_tiles;
@@ -358,12 +366,13 @@ void act8_wgrad_kernel(Product p) {
     *(float8*)&part[ry * kTN + cy] = sum;
     __syncthreads();
     const int64_t n = n0 + threadIdx.x;
-    if (threadIdx.x < kTN && n < p.n) {
+    if (threadIdx.x < kTN && n < p.part.n1) {
       float v = 0.f;
       for (int r = 0; r < kThreads * 8 / kTN; r++)
         v += part[r * kTN + threadIdx.x];
       if (p.slices > 1)
-        p.bias_partial[blockIdx.y * p.n + n] = v;
+        p.bias_partial[blockIdx.y * (p.part.n1 - p.part.n0) + n - p.part.n0] =
+            v;
       else
         ((O*)p.db)[n] = (O)v;
     }
@@ -372,7 +381,14 @@ void act8_wgrad_kernel(Product p) {
   float* out = (float*)lds + wave * 32 * kPitch;
   const int er = lane / (FK * 4), ec = lane % (FK * 4) * kVec;
   const int64_t ek = k0 + wk + ec;
-  const int em = p.k - ek < kVec ? (int)(p.k - ek) : kVec;
+  const int em = p.part.k1 - ek < kVec ? (int)(p.part.k1 - ek) : kVec;
+  // where the results go: dW, or the slice's part of it
+  const bool sliced = p.slices > 1;
+  const int64_t pitch = sliced ? p.part.k1 - p.part.k0 : p.k;
+  const int64_t origin =
+      sliced ? (blockIdx.y * (p.part.n1 - p.part.n0) - p.part.n0) * pitch -
+                   p.part.k0
+             : 0;
 #pragma unroll
   for (int bi = 0; bi < FN; bi++) {
 #pragma unroll
@@ -387,34 +403,47 @@ void act8_wgrad_kernel(Product p) {
     for (int r = er; r < 32; r += 16 / FK) {
       const int64_t n = n0 + wn + bi * 32 + r;
       const float8 v = *(const float8*)&out[r * kPitch + ec];
-      if (n >= p.n || em <= 0) continue;
-      if (p.slices > 1)
-        store_upto(p.partial + (blockIdx.y * p.n + n) * p.k + ek, v, em);
+      if (n >= p.part.n1 || em <= 0) continue;
+      const int64_t to = origin + n * pitch + ek;
+      if (sliced)
+        store_upto(p.partial + to, v, em);
       else
-        store_upto((O*)p.dw + n * p.k + ek, v, em);
+        store_upto((O*)p.dw + to, v, em);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
 }
 
-// dW and db from the slices' sums, in their order.
+// The part's dW and db from the slices' sums, in their order.
 template <typename O>
-__global__ __launch_bounds__(kThreads) void wgrad_join_kernel(
-    const float* partial, const float* bias, int slices, int64_t count,
-    int64_t n, O* dw, O* db) {
-  const int64_t step = (int64_t)gridDim.x * kThreads * kVec;
-  const int64_t first = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kVec;
-  auto join = [&](const float* parts, int64_t i, int64_t count, O* out) {
-    const int m = (int)(count - i < kVec ? count - i : kVec);
+__global__ __launch_bounds__(kThreads) void wgrad_join_kernel(Product p) {
+  const uint32_t step = gridDim.x * kThreads;
+  const uint32_t first = blockIdx.x * kThreads + threadIdx.x;
+  auto join = [&](const float* parts, int64_t each, int m) {
     float8 v = 0.f;
 #pragma unroll 4
-    for (int s = 0; s < slices; s++) v += load_upto(parts + s * count + i, m);
-    store_upto(out + i, v, m);
+    for (int s = 0; s < p.slices; s++) v += load_upto(parts + s * each, m);
+    return v;
   };
-  for (int64_t i = first; i < count; i += step) join(partial, i, count, dw);
-  if (db)
-    for (int64_t i = first; i < n; i += step) join(bias, i, n, db);
+  const uint32_t rows = (uint32_t)(p.part.n1 - p.part.n0);
+  const uint32_t cols = (uint32_t)(p.part.k1 - p.part.k0);
+  // whole rows of dW are one long row
+  const uint32_t width = cols == p.k ? rows * cols : cols;
+  const uint32_t vecs = (width + kVec - 1) / kVec;
+  const uint32_t items = cols == p.k ? vecs : rows * vecs;
+  for (uint32_t i = first; i < items; i += step) {
+    const uint32_t r = i / vecs, c = i % vecs * kVec;
+    const int m = width - c < kVec ? (int)(width - c) : kVec;
+    store_upto((O*)p.dw + (p.part.n0 + r) * p.k + p.part.k0 + c,
+               join(p.partial + (int64_t)r * cols + c, (int64_t)rows * cols, m),
+               m);
+  }
+  if (!p.db) return;
+  for (uint32_t i = first * kVec; i < rows; i += step * kVec) {
+    const int m = rows - i < kVec ? (int)(rows - i) : kVec;
+    store_upto((O*)p.db + p.part.n0 + i, join(p.bias_partial + i, rows, m), m);
+  }
 }
 
 // Gradients that the product cannot read as they are, laid out anew: rows
@@ -456,51 +485,99 @@ __global__ __launch_bounds__(kThreads) void layout_kernel(
   }
 }
 
+// How a part is computed: the tiles' shape, and the number of slices that the
+// rows are cut in.
+struct Shape {
+  Part part;
+  bool big;
+  int slices, slice_tiles;
+  double time;  // us, by the model
+};
+
 struct Plan {
-  bool big, laid_out;
-  int planes, slices, slice_tiles, xtiles, ntiles, ktiles;
+  bool laid_out;
+  int planes, xtiles, parts;
+  Shape shape[2];
   int64_t pitch;
   size_t laid_bytes, partial_bytes, bias_bytes;
 };
 
 size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
 
-// The tiles' shape and the number of slices that the rows are cut in, by the
-// time that they take, in us, from measurements of bf16 products with 64 to
-// 16384 rows and 64 to 8192 columns (the model is within 15% of them).
+// A part's shape and slices, by the time that they take, from measurements of
+// products with 32 to 16384 rows and 64 to 25088 columns (the model is within
+// 15% of them).
 //
 // Tiles of 256 by 256, one workgroup to a compute unit, need half of the LDS
-// reads that tiles of 128 by 128 do for the same work (1.45 us for 64 rows, or
-// 0.36 for a quarter of it, against 0.62 alone and 1.05 for two that share a
-// compute unit), but leave more of a small dW's edge empty and cut it in
-// fewer pieces: 2048 x 2048 x 2048 takes 27 us with the small ones and 41 with
-// the large, 4096 x 4096 x 4096 150 and 113.  Slices fill compute units that
-// too few tiles leave idle and cost a second pass over their sums: 16384 x
-// 256 x 256 takes 160 us in one slice and 21 in 16.
-void pick_shape(const Act8Wgrad& a, Plan& p) {
-  const int64_t tiles = (int64_t)p.planes * p.xtiles;
-  double best = 0;
+// reads that tiles of 128 by 128 do for the same work (1.5 us for 64 rows, or
+// 0.38 for a quarter of it, against 0.62 alone and 1.05 for two that share a
+// compute unit).  But they leave more of a small dW's edge empty, cut it in
+// fewer pieces, and nothing runs beside their start and their results' way out
+// (9 us, or 14.5 with fp32 results, against 4 and 6.5): 2048 x 2048 x 2048
+// takes 27 us with the small ones and 41 with the large, 64 x 4096 x 25088 57
+// and 71, 4096 x 4096 x 4096 150 and 113.  Small ones do not wait for each
+// other's rounds.  Slices fill compute units that too few tiles leave idle and
+// cost a second pass over their sums: 16384 x 256 x 256 takes 160 us in one
+// slice and 21 in 16.
+double tiles_time(bool big, bool f32, int64_t groups, int tiles) {
+  const double rounds = (double)groups / (big ? kUnits : 2 * kUnits);
+  const double tile = big ? 1.5 : groups > kUnits ? 1.05 : 0.62;
+  const double ends = big ? (f32 ? 14.5 : 9) : (f32 ? 6.5 : 4);
+  return (!big && rounds > 4 ? rounds : ceil(rounds)) * (tiles * tile + ends);
+}
+
+Shape pick_shape(const Part& part, bool f32, int tiles) {
+  const int64_t rows = part.n1 - part.n0, cols = part.k1 - part.k0;
+  Shape s = {};
   for (int big = 0; big < 2; big++) {
     const int size = big ? 256 : 128;
-    const int64_t nt = (a.n + size - 1) / size, kt = (a.k + size - 1) / size;
-    for (int64_t cut = 1; cut <= 512 && cut <= tiles;
-         cut += 1 + cut / 16) {
-      const int64_t each = (tiles + cut - 1) / cut;
+    const int64_t nt = (rows + size - 1) / size, kt = (cols + size - 1) / size;
+    for (int cut = 1; cut <= 512 && cut <= tiles; cut += 1 + cut / 16) {
+      const int each = (tiles + cut - 1) / cut;
       if ((tiles + each - 1) / each != cut) continue;
-      const double groups = (double)nt * kt * cut;
-      if (cut > 1 && groups > 1024) break;
-      const double rounds = ceil(groups / (big ? 256 : 512));
-      const double tile = big ? 1.45 : groups > 256 ? 1.05 : 0.62;
-      double t = rounds * (each * tile + (big ? 9 : 5));
-      if (cut > 1) t += 4 + cut * (double)a.n * a.k * 1e-6;
-      if (best > 0 && t >= best) continue;
-      best = t;
-      p.big = big;
-      p.ntiles = (int)nt;
-      p.ktiles = (int)kt;
-      p.slices = (int)cut;
-      p.slice_tiles = (int)each;
+      if (cut > 1 && nt * kt * cut > 1024) break;
+      double t = tiles_time(big, f32, nt * kt * cut, each);
+      if (cut > 1) t += 4 + cut * (double)rows * cols * 1e-6;
+      if (s.time > 0 && t >= s.time) continue;
+      s = {part, (bool)big, cut, each, t};
+      s.part.ntiles = (int)nt;
+      s.part.ktiles = (int)kt;
     }
+  }
+  return s;
+}
+
+// Large tiles that fill the compute units a whole number of times, and the
+// columns or rows of dW behind them as a part of its own, where that is
+// quicker: a last round of a few large tiles takes as long as a full one.  bf16
+// products of 4096 x 4352 x 4352 took 202 us without parts and take 150, 8192
+// x 2048 x 8448 335 and 240, 12000 x 6000 x 6000 848 and 748.
+void pick_parts(const Act8Wgrad& a, Plan& p) {
+  const int tiles = p.planes * p.xtiles;
+  const int64_t nt = (a.n + 255) / 256, kt = (a.k + 255) / 256;
+  p.parts = 1;
+  const bool f32 = p.planes > 1;
+  p.shape[0] = pick_shape({0, a.n, 0, a.k}, f32, tiles);
+  double best = p.shape[0].time;
+  const int64_t full = nt * kt / kUnits;  // rounds
+  if (full < 1 || full > 64 || nt * kt % kUnits == 0) return;
+  for (int along_k = 0; along_k < 2; along_k++) {
+    const int64_t other = along_k ? nt : kt;
+    const int64_t own = full * kUnits / other;  // columns or rows of tiles
+    if (own < 1) continue;
+    Part first = {0, a.n, 0, a.k, (int)nt, (int)kt}, rest = first;
+    if (along_k)
+      first.k1 = rest.k0 = own * 256, first.ktiles = (int)own;
+    else
+      first.n1 = rest.n0 = own * 256, first.ntiles = (int)own;
+    const double time =
+        tiles_time(true, f32, (int64_t)first.ntiles * first.ktiles, tiles);
+    const Shape s = pick_shape(rest, f32, tiles);
+    if (time + s.time + 2 >= best) continue;
+    best = time + s.time + 2;
+    p.parts = 2;
+    p.shape[0] = {first, true, 1, tiles, time};
+    p.shape[1] = s;
   }
 }
 
@@ -515,19 +592,22 @@ Plan plan_of(const Act8Wgrad& a) {
   if (p.laid_out)
     p.laid_bytes =
         round256((size_t)p.planes * p.xtiles * kTM * p.pitch * 2);
-  pick_shape(a, p);
-  if (p.slices > 1) {
-    p.partial_bytes = round256((size_t)p.slices * a.n * a.k * sizeof(float));
-    p.bias_bytes = round256((size_t)p.slices * a.n * sizeof(float));
+  pick_parts(a, p);
+  const Shape& s = p.shape[p.parts - 1];  // the only one that has slices
+  if (s.slices > 1) {
+    const size_t rows = (size_t)s.slices * (s.part.n1 - s.part.n0);
+    p.partial_bytes =
+        round256(rows * (s.part.k1 - s.part.k0) * sizeof(float));
+    p.bias_bytes = round256(rows * sizeof(float));
   }
   return p;
 }
 
 template <typename T, typename O>
-void launch_product(const Plan& plan, const Product& p, hipStream_t stream) {
-  const dim3 grid((uint32_t)(plan.ntiles * plan.ktiles),
-                  (uint32_t)plan.slices);
-  if (plan.big)
+void launch_product(const Shape& s, const Product& p, hipStream_t stream) {
+  const dim3 grid((uint32_t)(s.part.ntiles * s.part.ktiles),
+                  (uint32_t)s.slices);
+  if (s.big)
     launch(act8_wgrad_kernel<T, O, 4, 4>, grid, kThreads, stream, p);
   else
     launch(act8_wgrad_kernel<T, O, 2, 2>, grid, kThreads, stream, p);
@@ -550,9 +630,12 @@ hipError_t act8_wgrad(const Act8Wgrad& a, hipStream_t stream) {
   if (a.m == 0 || a.n == 0 || a.k == 0) return hipSuccess;
   if (a.n > kAct8MaxCols || a.pitch > kAct8MaxCols) return hipErrorInvalidValue;
   const Plan plan = plan_of(a);
-  if ((int64_t)plan.ntiles * plan.ktiles * plan.slices > (1 << 23) ||
-      plan.slices > 65535)
-    return hipErrorInvalidValue;
+  for (int i = 0; i < plan.parts; i++) {
+    const Shape& s = plan.shape[i];
+    if ((int64_t)s.part.ntiles * s.part.ktiles * s.slices > (1 << 23) ||
+        s.slices > 65535)
+      return hipErrorInvalidValue;
+  }
   char* ws = (char*)a.workspace;
   const int64_t laid_rows = (int64_t)plan.xtiles * kTM;
   Product p = {};
@@ -572,14 +655,8 @@ hipError_t act8_wgrad(const Act8Wgrad& a, hipStream_t stream) {
             (int)((a.m - last) * a.pitch / kAct8Group)};
   p.xtiles = plan.xtiles;
   p.tiles = plan.planes * plan.xtiles;
-  p.slices = plan.slices;
-  p.slice_tiles = plan.slice_tiles;
-  p.ntiles = plan.ntiles;
-  p.ktiles = plan.ktiles;
-  p.n = a.n;
   p.k = a.k;
   p.dw = a.dw;
-  p.db = a.db;
   p.partial = (float*)(ws + plan.laid_bytes);
   p.bias_partial = (float*)(ws + plan.laid_bytes + plan.partial_bytes);
   with_type(a.type, [&](auto* t) {
@@ -589,11 +666,20 @@ hipError_t act8_wgrad(const Act8Wgrad& a, hipStream_t stream) {
       launch(layout_kernel<T, P>, flat_grid(laid_rows * plan.pitch / kVec),
              kThreads, stream, (const T*)a.dy, a.dstride, a.m, a.n, (P*)ws,
              laid_rows, plan.pitch);
-    launch_product<P, T>(plan, p, stream);
-    if (plan.slices > 1)
-      launch(wgrad_join_kernel<T>, flat_grid(a.n * a.k / kVec + 1), kThreads,
-             stream, (const float*)p.partial, (const float*)p.bias_partial,
-             plan.slices, a.n * a.k, a.n, (T*)a.dw, (T*)a.db);
+    for (int i = 0; i < plan.parts; i++) {
+      const Shape& s = plan.shape[i];
+      p.part = s.part;
+      p.slices = s.slices;
+      p.slice_tiles = s.slice_tiles;
+      p.db = s.part.k0 == 0 ? a.db : nullptr;
+      launch_product<P, T>(s, p, stream);
+      if (s.slices > 1)
+        launch(wgrad_join_kernel<T>,
+               flat_grid((s.part.n1 - s.part.n0) * (s.part.k1 - s.part.k0) /
+                             kVec +
+                         1),
+               kThreads, stream, p);
+    }
   });
   return hipGetLastError();
 }

@@ -153,6 +153,14 @@ def test_wgrad_long(dtype, m, n, k):
     wgrad(m, n, k, dtype)
 
 
+@pytest.mark.parametrize("dtype,m,n,k", [
+    (BF, 1000, 2048, 8448), (F32, 700, 2048, 8440), (BF, 1000, 8448, 2048),
+    (F32, 130, 8449, 2050), (HF, 300, 4401, 4350), (BF, 600, 4352, 4352)])
+def test_wgrad_of_uneven_sizes(dtype, m, n, k):
+    """A few tiles more than a round of the chip's: dW is computed in parts."""
+    wgrad(m, n, k, dtype, seed=n)
+
+
 def test_wgrad_strides():
     big = rows((200, 150), BF, 3, wild=False).cuda()
     for dy in (big[:, 3:77], big[::2, 1:], big.t(), big[:1].expand(90, 150),
