@@ -9,8 +9,14 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
+#include <array>
+#include <memory>
+#include <mutex>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -21,7 +27,6 @@ namespace baguanet {
 namespace {
 
 using torch::Tensor;
-using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using OptTensor = std::optional<Tensor>;
 
@@ -70,9 +75,42 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors) {
 
 const Tensor* get(const OptTensor& t) { return t ? &*t : nullptr; }
 
-void no_double_backward(const char* op) {
-  TORCH_CHECK(!at::GradMode::is_enabled(), op,
-              ": its gradient cannot be differentiated again");
+// An operator's backward pass: a node of the graph that keeps N tensors.  As a
+// node of its own it has its numbers as members; through torch's Function, with
+// its context of named values, a call with a gradient took 5 us longer.
+template <size_t N>
+class OpNode : public torch::autograd::Node {
+ public:
+  // Only once t has been written: a hook may copy it here.
+  void keep(size_t i, const Tensor& t) {
+    saved_[i] = torch::autograd::SavedVariable(t, false);
+  }
+
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    for (auto& s : saved_) s.reset_data();
+  }
+
+ protected:
+  std::array<Tensor, N> kept(const char* op) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), op,
+                ": its gradient cannot be differentiated again");
+    const std::lock_guard<std::mutex> lock(mutex_);
+    std::array<Tensor, N> t;
+    for (size_t i = 0; i < N; i++) t[i] = saved_[i].unpack();
+    return t;
+  }
+
+ private:
+  std::array<torch::autograd::SavedVariable, N> saved_;
+};
+
+// A node that gives gradients to `inputs`, in their order.
+template <typename Op, typename... T>
+std::shared_ptr<Op> make_node(const T&... inputs) {
+  std::shared_ptr<Op> node(new Op(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+  return node;
 }
 
 // A tensor as rows of its last dimension: unit stride within a row and one
@@ -108,8 +146,6 @@ Tensor empty_bytes(size_t bytes, const Tensor& like) {
   return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
 }
 
-Tensor or_undefined(const OptTensor& t) { return t ? *t : Tensor(); }
-
 // ---------------------------------------------------------------------------
 // embedding
 
@@ -136,31 +172,23 @@ Tensor lookup(const Tensor& weight, const Tensor& tok, double scale,
   return out;
 }
 
-struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& weight,
-                        const Tensor& tok, double scale, int64_t padding,
-                        int64_t out_type) {
-    ctx->save_for_backward({tok});
-    ctx->saved_data["vocab"] = weight.size(0);
-    ctx->saved_data["scale"] = scale;
-    ctx->saved_data["padding"] = padding;
-    ctx->saved_data["type"] = (int64_t)weight.scalar_type();
-    return lookup(weight, tok, scale, (at::ScalarType)out_type);
-  }
+struct EmbeddingNode : OpNode<1> {
+  int64_t vocab, padding;
+  double scale;
+  at::ScalarType type;
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    no_double_backward("embedding");
-    const Tensor tok = ctx->get_saved_variables()[0];
+  std::string name() const override { return "EmbeddingBackward"; }
+
+  variable_list apply(variable_list&& grads) override {
+    const Tensor tok = kept("embedding")[0];
+    if (!grads[0].defined()) return {Tensor()};
     const Rows dout = as_rows(grads[0]);
     const c10::OptionalDeviceGuard guard(dout.t.device());
     EmbeddingBwd a = {};
-    a.vocab = ctx->saved_data["vocab"].toInt();
+    a.vocab = vocab;
     a.dim = dout.t.size(-1);
     a.n = tok.numel();
-    Tensor dw = at::empty(
-        {a.vocab, a.dim},
-        dout.t.options().dtype(
-            (at::ScalarType)ctx->saved_data["type"].toInt()));
+    Tensor dw = at::empty({a.vocab, a.dim}, dout.t.options().dtype(type));
     const Tensor ws =
         empty_bytes(embedding_workspace(a.vocab, a.dim, a.n), dout.t);
     a.dout = dout.t.data_ptr();
@@ -168,13 +196,13 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
     a.dweight = dw.data_ptr();
     a.workspace = ws.data_ptr();
     a.dstride = dout.stride;
-    a.padding = ctx->saved_data["padding"].toInt();
-    a.scale = (float)ctx->saved_data["scale"].toDouble();
+    a.padding = padding;
+    a.scale = (float)scale;
     a.tok64 = tok.scalar_type() == at::kLong;
     a.dtype = elem(dout.t.scalar_type());
-    a.wtype = elem(dw.scalar_type());
+    a.wtype = elem(type);
     check_launch(embedding_backward(a, stream_of(dw)), "embedding backward");
-    return {dw, Tensor(), Tensor(), Tensor(), Tensor()};
+    return {dw};
   }
 };
 
@@ -205,7 +233,16 @@ Tensor embedding(const Tensor& weight, const Tensor& tokens, double scale,
   check_device(tokens, weight, op, "tokens");
   const Tensor tok = tokens.contiguous();
   if (!wants_grad({&weight})) return lookup(weight, tok, scale, out);
-  return EmbeddingFn::apply(weight, tok, scale, padding, (int64_t)out);
+  const auto node = make_node<EmbeddingNode>(weight);
+  node->vocab = vocab;
+  node->padding = padding;
+  node->scale = scale;
+  node->type = weight.scalar_type();
+  node->keep(0, tok);
+  const at::NoGradGuard no_grad;
+  Tensor y = lookup(weight, tok, scale, out);
+  torch::autograd::set_history(y, node);
+  return y;
 }
 
 // ---------------------------------------------------------------------------
@@ -267,48 +304,16 @@ std::tuple<Tensor, Tensor> run_norm(const NormArgs& n, const Tensor& stats) {
   return {y, h};
 }
 
-struct NormFn : torch::autograd::Function<NormFn> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& x,
-                               const OptTensor& branch, const OptTensor& gate,
-                               const OptTensor& post, const OptTensor& pre,
-                               double residual_scale, double branch_scale,
-                               double eps, int64_t gmode, int64_t group_rows,
-                               bool want_h) {
-    const NormArgs n = {x,
-                        or_undefined(branch),
-                        or_undefined(gate),
-                        or_undefined(post),
-                        or_undefined(pre),
-                        residual_scale,
-                        branch_scale,
-                        eps,
-                        (Gate)gmode,
-                        group_rows,
-                        want_h};
-    const Tensor stats =
-        at::empty({2, rows_of(x)}, x.options().dtype(at::kFloat));
-    auto [y, h] = run_norm(n, stats);
-    ctx->set_materialize_grads(false);
-    ctx->save_for_backward(
-        {want_h ? x : Tensor(), n.branch, n.gate, n.post, n.pre, stats});
-    ctx->saved_data["scales"] = c10::complex<double>(residual_scale,
-                                                     branch_scale);
-    ctx->saved_data["group_rows"] = group_rows;
-    const auto needs = [](const Tensor& t) {
-      return t.defined() && t.requires_grad();
-    };
-    ctx->saved_data["gate"] = gmode | needs(n.gate) << 4 | needs(n.post) << 5 |
-                              needs(n.pre) << 6;
-    variable_list out;
-    if (y.defined()) out.push_back(y);
-    if (h.defined()) out.push_back(h);
-    return out;
-  }
+struct NormNode : OpNode<6> {
+  double residual_scale, branch_scale;
+  Gate gmode;
+  int64_t group_rows;
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    no_double_backward("residual norm");
-    variable_list out(11);
-    const auto saved = ctx->get_saved_variables();
+  std::string name() const override { return "GatedResidualNormBackward"; }
+
+  variable_list apply(variable_list&& grads) override {
+    const auto saved = kept("residual norm");
+    variable_list out(5);
     const Tensor &x = saved[0], &branch = saved[1], &gate = saved[2],
                  &post = saved[3], &pre = saved[4];
     const float* stats = saved[5].data_ptr<float>();
@@ -326,14 +331,10 @@ struct NormFn : torch::autograd::Function<NormFn> {
     a.rows = rows_of(some);
     a.dim = some.size(-1);
     a.type = elem(some.scalar_type());
-    const auto scales = ctx->saved_data["scales"].toComplexDouble();
-    const int64_t flags = ctx->saved_data["gate"].toInt();
-    const bool needs[3] = {(flags >> 4 & 1) != 0, (flags >> 5 & 1) != 0,
-                           (flags >> 6 & 1) != 0};
-    a.residual_scale = (float)scales.real();
-    a.branch_scale = (float)scales.imag();
-    a.gmode = (Gate)(flags & 15);
-    a.group_rows = ctx->saved_data["group_rows"].toInt();
+    a.residual_scale = (float)residual_scale;
+    a.branch_scale = (float)branch_scale;
+    a.gmode = gmode;
+    a.group_rows = group_rows;
     Rows xr, br, dyr, dhr;
     Tensor dx = at::empty(some.sizes(), some.options());
     a.dx = dx.data_ptr();
@@ -354,7 +355,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
       if (pre.defined()) {
         a.pre = pre.data_ptr();
         a.pre32 = pre.scalar_type() == at::kFloat;
-        if (needs[2]) {
+        if (task_should_compute_output(4)) {
           dpre = at::empty(pre.sizes(), pre.options());
           a.dpre = dpre.data_ptr();
         }
@@ -369,7 +370,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
       if (gate.defined()) {
         a.gate = gate.data_ptr();
         a.gate32 = gate.scalar_type() == at::kFloat;
-        if (needs[0]) {
+        if (task_should_compute_output(2)) {
           dgate = at::empty(gate.sizes(), gate.options());
           a.dgate = dgate.data_ptr();
         }
@@ -378,7 +379,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
         a.post = post.data_ptr();
         a.post32 = post.scalar_type() == at::kFloat;
         a.rbranch = stats;
-        if (needs[1]) {
+        if (task_should_compute_output(3)) {
           dpost = at::empty(post.sizes(), post.options());
           a.dpost = dpost.data_ptr();
         }
@@ -400,6 +401,28 @@ struct NormFn : torch::autograd::Function<NormFn> {
   }
 };
 
+// y and h as run_norm gives them, with their place in the graph.
+std::tuple<Tensor, Tensor> norm_with_grad(const NormArgs& n) {
+  const auto node = make_node<NormNode>(n.x, n.branch, n.gate, n.post, n.pre);
+  node->residual_scale = n.residual_scale;
+  node->branch_scale = n.branch_scale;
+  node->gmode = n.gmode;
+  node->group_rows = n.group_rows;
+  const at::NoGradGuard no_grad;
+  const Tensor stats =
+      at::empty({2, rows_of(n.x)}, n.x.options().dtype(at::kFloat));
+  auto [y, h] = run_norm(n, stats);
+  if (n.want_h) node->keep(0, n.x);
+  node->keep(1, n.branch);
+  node->keep(2, n.gate);
+  node->keep(3, n.post);
+  node->keep(4, n.pre);
+  node->keep(5, stats);
+  if (y.defined()) torch::autograd::set_history(y, node);
+  if (h.defined()) torch::autograd::set_history(h, node);
+  return {y, h};
+}
+
 void check_norm_input(const Tensor& x, const char* op, const char* name) {
   check_act(x, op, name);
   TORCH_CHECK(x.dim() >= 1, op, ": ", name, " must have rows, not be a scalar");
@@ -420,8 +443,8 @@ void check_norm_weight(const OptTensor& w, const Tensor& x, const char* op,
               " must be [", x.size(-1), "], not ", w->sizes());
 }
 
-OptTensor contiguous(const OptTensor& t) {
-  return t ? OptTensor(t->contiguous()) : OptTensor();
+Tensor contiguous(const OptTensor& t) {  // undefined where it is not given
+  return t ? t->contiguous() : Tensor();
 }
 
 Tensor rms_norm(const Tensor& x, const OptTensor& weight, double eps) {
@@ -431,13 +454,10 @@ Tensor rms_norm(const Tensor& x, const OptTensor& weight, double eps) {
   TORCH_CHECK(eps >= 0, op, ": eps must not be negative");
   check_device(x, x, op, "x");
   if (weight) check_device(*weight, x, op, "weight");
-  const OptTensor w = contiguous(weight);
-  if (!wants_grad({&x, get(w)}))
-    return std::get<1>(run_norm({x, {}, {}, {}, or_undefined(w), 1.0, 1.0, eps,
-                                 Gate::kNone, 1, true},
-                                Tensor()));
-  return NormFn::apply(x, OptTensor(), OptTensor(), OptTensor(), w, 1.0, 1.0,
-                       eps, (int64_t)Gate::kNone, int64_t(1), true)[0];
+  const NormArgs n = {x,   {},  {},  {},          contiguous(weight), 1.0,
+                      1.0, eps, Gate::kNone, 1, true};
+  return std::get<1>(wants_grad({&x, &n.pre}) ? norm_with_grad(n)
+                                              : run_norm(n, Tensor()));
 }
 
 std::tuple<Tensor, OptTensor> gated_residual_norm(
@@ -458,7 +478,7 @@ std::tuple<Tensor, OptTensor> gated_residual_norm(
   const int64_t dim = x.size(-1), rows = rows_of(x);
   Gate mode = Gate::kNone;
   int64_t group_rows = rows > 0 ? rows : 1;
-  OptTensor g;
+  Tensor g;
   if (gate) {
     check_act(*gate, op, "gate");
     TORCH_CHECK(gate->scalar_type() == at::kFloat ||
@@ -500,19 +520,21 @@ std::tuple<Tensor, OptTensor> gated_residual_norm(
   if (gate) check_device(*gate, x, op, "gate");
   if (post_weight) check_device(*post_weight, x, op, "post_weight");
   if (pre_weight) check_device(*pre_weight, x, op, "pre_weight");
-  const OptTensor post = contiguous(post_weight), pre = contiguous(pre_weight);
-  const bool want_h = pre.has_value();
-  if (!wants_grad({&x, &branch, get(g), get(post), get(pre)})) {
-    auto [y, h] = run_norm({x, branch, or_undefined(g), or_undefined(post),
-                            or_undefined(pre), residual_scale, branch_scale,
-                            eps, mode, group_rows, want_h},
-                           Tensor());
-    return {y, want_h ? OptTensor(h) : OptTensor()};
-  }
-  auto out = NormFn::apply(x, branch, g, post, pre, residual_scale,
-                           branch_scale, eps, (int64_t)mode, group_rows,
-                           want_h);
-  return {out[0], want_h ? OptTensor(out[1]) : OptTensor()};
+  const NormArgs n = {x,
+                      branch,
+                      g,
+                      contiguous(post_weight),
+                      contiguous(pre_weight),
+                      residual_scale,
+                      branch_scale,
+                      eps,
+                      mode,
+                      group_rows,
+                      pre_weight.has_value()};
+  auto [y, h] = wants_grad({&x, &branch, &g, &n.post, &n.pre})
+                    ? norm_with_grad(n)
+                    : run_norm(n, Tensor());
+  return {y, n.want_h ? OptTensor(h) : OptTensor()};
 }
 
 // ---------------------------------------------------------------------------
@@ -686,47 +708,37 @@ Tensor flat_linear(const Tensor& x, const Tensor& weight,
                    const OptTensor& bias) {
   auto sizes = x.sizes().vec();
   sizes.back() = weight.size(0);
-  return at::linear(x.reshape({rows_of(x), x.size(-1)}), weight, bias)
-      .view(sizes);
+  return at::_unsafe_view(
+      at::linear(x.reshape({rows_of(x), x.size(-1)}), weight, bias), sizes);
 }
 
 // A linear layer whose input is kept in 8 bits.  Its two plain products, y
 // and dx, are the library's, as in torch.nn.Linear; the weight gradient is
 // taken from the codes.
-struct LinearAct8Fn : torch::autograd::Function<LinearAct8Fn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x,
-                        const Tensor& weight, const OptTensor& bias) {
-    Tensor codes, exps;
-    const bool grad_b = bias && bias->requires_grad();
-    if (weight.requires_grad()) std::tie(codes, exps) = pack_rows(x);
-    ctx->save_for_backward(
-        {x.requires_grad() ? weight : Tensor(), codes, exps});
-    ctx->saved_data["needs"] = std::vector<int64_t>{
-        x.requires_grad(), weight.requires_grad(), grad_b};
-    ctx->saved_data["k"] = x.size(-1);
-    return flat_linear(x, weight, bias);
-  }
+struct LinearAct8Node : OpNode<3> {
+  int64_t k;
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    no_double_backward("linear_act8");
+  std::string name() const override { return "LinearAct8Backward"; }
+
+  variable_list apply(variable_list&& grads) override {
     const c10::impl::ExcludeDispatchKeyGuard own_types(
         c10::autocast_dispatch_keyset);
-    const auto saved = ctx->get_saved_variables();
-    const auto needs = ctx->saved_data["needs"].toIntVector();
+    const auto saved = kept("linear_act8");
+    variable_list out(3);
+    if (!grads[0].defined()) return out;
     const Tensor& dy = grads[0];
     const c10::OptionalDeviceGuard guard(dy.device());
-    variable_list out(3);
-    if (needs[0]) {
+    if (task_should_compute_output(0)) {
       auto sizes = dy.sizes().vec();
       sizes.back() = saved[0].size(1);
       out[0] = at::mm(dy.reshape({rows_of(dy), dy.size(-1)}), saved[0])
                    .view(sizes);
     }
-    if (needs[1])
+    const bool bias = task_should_compute_output(2);
+    if (task_should_compute_output(1))
       std::tie(out[1], out[2]) =
-          wgrad_rows(dy, saved[1], saved[2], ctx->saved_data["k"].toInt(),
-                     needs[2]);
-    else if (needs[2])
+          wgrad_rows(dy, saved[1], saved[2], k, bias);
+    else if (bias)
       out[2] = bias_rows(dy);
     return out;
   }
@@ -762,7 +774,18 @@ Tensor linear_act8(const Tensor& x, const Tensor& weight,
   const c10::OptionalDeviceGuard guard(x.device());
   if (!wants_grad({&x, &weight, get(bias)}))
     return flat_linear(x, weight, bias);
-  return LinearAct8Fn::apply(x, weight, bias);
+  const auto node = make_node<LinearAct8Node>(x, weight, bias);
+  node->k = x.size(-1);
+  const at::NoGradGuard no_grad;
+  if (x.requires_grad()) node->keep(0, weight);
+  if (weight.requires_grad()) {
+    const auto [codes, exps] = pack_rows(x);
+    node->keep(1, codes);
+    node->keep(2, exps);
+  }
+  Tensor y = flat_linear(x, weight, bias);
+  torch::autograd::set_history(y, node);
+  return y;
 }
 
 // silu(a) * b, and the copies of a and b where they are defined.
@@ -788,20 +811,12 @@ Tensor run_silu(const Tensor& x, const Tensor& codes, const Tensor& exps) {
   return out;
 }
 
-struct SiluAct8Fn : torch::autograd::Function<SiluAct8Fn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x) {
-    const c10::OptionalDeviceGuard guard(x.device());
-    const int64_t rows = rows_of(x), pitch = pitch_of(x.size(-1) / 2);
-    const auto bytes = x.options().dtype(at::kByte);
-    const Tensor codes = at::empty({rows, 2 * pitch}, bytes);
-    const Tensor exps = at::empty({rows, 2 * pitch / kAct8Group}, bytes);
-    ctx->save_for_backward({codes, exps});
-    return run_silu(x, codes, exps);
-  }
+struct SiluAct8Node : OpNode<2> {
+  std::string name() const override { return "SiluMulAct8Backward"; }
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    no_double_backward("silu_mul_act8");
-    const auto saved = ctx->get_saved_variables();
+  variable_list apply(variable_list&& grads) override {
+    const auto saved = kept("silu_mul_act8");
+    if (!grads[0].defined()) return {Tensor()};
     const Rows dr = as_rows(grads[0]);
     const c10::OptionalDeviceGuard guard(dr.t.device());
     SiluAct8 p = {};
@@ -831,7 +846,18 @@ Tensor silu_mul_act8(const Tensor& x) {
               x.size(-1), " columns");
   check_device(x, x, op, "x");
   if (!wants_grad({&x})) return run_silu(x, Tensor(), Tensor());
-  return SiluAct8Fn::apply(x);
+  const auto node = make_node<SiluAct8Node>(x);
+  const at::NoGradGuard no_grad;
+  const c10::OptionalDeviceGuard guard(x.device());
+  const int64_t rows = rows_of(x), pitch = pitch_of(x.size(-1) / 2);
+  const auto bytes = x.options().dtype(at::kByte);
+  const Tensor codes = at::empty({rows, 2 * pitch}, bytes);
+  const Tensor exps = at::empty({rows, 2 * pitch / kAct8Group}, bytes);
+  Tensor out = run_silu(x, codes, exps);
+  node->keep(0, codes);
+  node->keep(1, exps);
+  torch::autograd::set_history(out, node);
+  return out;
 }
 
 }  // namespace

@@ -234,3 +234,101 @@ def test_whole_step_in_a_graph():
         want = step()
         model.kept.clear()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def _each_operator():
+    """Every operator with a gradient, as a function of its leaves."""
+    from baguanet import ops
+
+    g = torch.Generator().manual_seed(5)
+
+    def leaf(*shape):
+        return torch.randn(*shape, generator=g).cuda().requires_grad_()
+
+    tok = torch.tensor([[3, 1, 3], [0, 2, 3]], device="cuda")
+    return [
+        (lambda w: ops.embedding(w, tok, 2.0), [leaf(5, 40)]),
+        (lambda x, w: ops.rms_norm(x, w), [leaf(6, 40), leaf(40)]),
+        (lambda x, o, gate, post, pre: ops.gated_residual_norm(
+            x, o, gate, post, pre)[1],
+         [leaf(6, 40), leaf(6, 40), leaf(40), leaf(40), leaf(40)]),
+        (lambda x, o, gate, post, pre: ops.gated_residual_norm(
+            x, o, gate, post, pre)[0],
+         [leaf(2, 3, 40), leaf(2, 3, 40), leaf(2, 1, 40), leaf(40), leaf(40)]),
+        (lambda x, w, b: ops.linear_act8(x, w, b),
+         [leaf(2, 3, 40), leaf(24, 40), leaf(24)]),
+        (lambda x: ops.silu_mul_act8(x), [leaf(6, 80)])]
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_each_gradient_alone(which):
+    """Asked for by itself, a gradient is the one of all together."""
+    f, leaves = _each_operator()[which]
+    y = f(*leaves)
+    dout = torch.randn_like(y)
+    used = torch.autograd.grad(y, leaves, dout, retain_graph=True,
+                               allow_unused=True)
+    for leaf, want in zip(leaves, used):
+        (got,) = torch.autograd.grad(y, leaf, dout, retain_graph=True,
+                                     allow_unused=True)
+        assert (got is None) == (want is None)
+        assert want is None or torch.equal(got, want)
+    # with only one of the leaves in the graph
+    for i, want in enumerate(used):
+        few = [t if i == j else t.detach() for j, t in enumerate(leaves)]
+        if want is not None:
+            (got,) = torch.autograd.grad(f(*few), leaves[i], dout)
+            assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_graph_is_torchs_own(which):
+    """Results changed in place, recomputed blocks, hooks on what is kept,
+    freed graphs: as with torch's operators."""
+    from torch.utils.checkpoint import checkpoint
+
+    f, leaves = _each_operator()[which]
+    y = f(*leaves)
+    dout = torch.randn_like(y)
+    want = torch.autograd.grad(y, leaves, dout, allow_unused=True)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, leaves, dout, allow_unused=True)
+
+    def same(y, dout=dout):
+        got = torch.autograd.grad(y, leaves, dout, allow_unused=True)
+        for a, b in zip(got, want):
+            assert (a is None) == (b is None)
+            assert a is None or torch.equal(a, b)
+
+    same(f(*leaves).mul_(2.0), dout / 2)
+    same(f(*leaves).view(-1).view(y.shape))
+    same(checkpoint(f, *leaves, use_reentrant=False))
+    count = []
+
+    def to_host(t):
+        count.append(t.numel())
+        return t.cpu()
+
+    with torch.autograd.graph.saved_tensors_hooks(to_host,
+                                                  lambda t: t.cuda()):
+        z = f(*leaves)
+    assert count
+    same(z)
+    for leaf in leaves:
+        leaf.grad = None
+    f(*leaves).backward(dout)
+    for leaf, b in zip(leaves, want):
+        assert (leaf.grad is None) == (b is None)
+        assert b is None or torch.equal(leaf.grad, b)
+
+
+def test_kept_tensors_are_guarded():
+    """A kept tensor that is changed before the backward pass is noticed."""
+    from baguanet import ops
+
+    w = torch.randn(40, device="cuda", requires_grad=True)
+    x = torch.randn(6, 40, device="cuda")
+    y = ops.rms_norm(x, w)
+    x.mul_(2.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
