@@ -157,12 +157,15 @@ __global__ __launch_bounds__(kRankBlock) void sort_rank_kernel(EmbeddingBwd a,
 
 // More tokens: least-significant-digit radix sort.  Each pass counts the
 // digits of every tile of tokens and places the tile's elements in order.
-// The tiles are cut so that there are at most 64: each of them then adds up
-// the counts of all for itself, and their scan needs no launch of its own.
+// The tiles are cut so that there are at most 64, or 128 from 131072 tokens on
+// and 256 from 524288 on: each of them then adds up the counts of all for
+// itself, and their scan needs no launch of its own.  (262144 tokens of 50000 x
+// 512: gradient 189 us with 64 and 173 with 128; 1000000 of 131072 x 64: 437
+// with 64, 354 with 128 and 327 with 256.)
 constexpr int kSortBlock = 256;
 constexpr int kSortWaves = kSortBlock / kWave;
 constexpr int kMaxBits = 10;         // of a digit: 1024 counters
-constexpr int64_t kMaxTiles = 64;
+constexpr int64_t kMaxTiles = 256;
 
 struct Tiles {
   int64_t size, count;  // elements of a tile, a multiple of kSortBlock
@@ -399,55 +402,43 @@ __global__ __launch_bounds__(kBlock) void embedding_sum_kernel(
     starts.chunk[atomicAdd(starts.count, 1)] = (int32_t)chunk;
 }
 
-// The runs that cross chunk borders, each summed from its parts by one
-// workgroup for a tile of columns: its threads look for the run's end
-// together, each of its teams adds up every so many of the parts, and the
-// teams' sums are added in their order.  Teams have 128 lanes at most, so
-// that the hundreds of parts of the most frequent token are shared by four
-// (18 us with 256 lanes, 13 with 128: 50000 x 2048 bf16, 16384 tokens).
+// The runs that cross chunk borders, for each a tile of columns at a time.  A
+// workgroup sums one from its parts: its threads look for the run's end
+// together, its teams add up every so many of the parts, and the teams' sums
+// are added in their order.  Teams have 128 lanes at most, so that the hundreds
+// of parts of the most frequent token are shared by four (18 us with 256
+// lanes, 13 with 128: 50000 x 2048 bf16, 16384 tokens).
+//
+// kMany: for many runs, most of a few parts.  A wave sums one of those alone
+// and adds its teams' sums pairwise, and the workgroup follows with the
+// others: 140 us without this and 60 with it at 1000000 tokens of 131072 x 64,
+// but 10 and 15 at 65536 tokens of 1000 x 64.
 constexpr int kJoinBlock = 512, kJoinBlocks = 1024;
 
-template <typename W, bool kTiny>
+template <typename W, bool kTiny, bool kMany>
 __global__ __launch_bounds__(kJoinBlock) void embedding_join_kernel(
     EmbeddingBwd a, Sorted s, Chunks ch, Starts starts, const float* partial) {
-  __shared__ int wave_end[kJoinBlock / kWave];
+  constexpr int kWaves = kJoinBlock / kWave, kRuns = kMany ? kWaves : 1;
+  constexpr int kLanes = kMany ? kWave : 128;
+  __shared__ int wave_end[kWaves], many[kRuns];
   __shared__ float joint[kJoinBlock * kVec];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const int tpr = ch.tpr < 128 ? ch.tpr : 128, teams = kJoinBlock / tpr;
+  const int tpr = ch.tpr < kLanes ? ch.tpr : kLanes;
   const int team = threadIdx.x / tpr, in = threadIdx.x % tpr;
+  const int teams = kJoinBlock / tpr;
   const int64_t tiles = (a.dim + tpr * kVec - 1) / (tpr * kVec);
-  const int64_t items = *starts.count * tiles;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int64_t chunk = starts.chunk[item / tiles];
-    const int32_t key = s.key[(chunk + 1) * ch.size - 1];
-    // chunks that begin with the key hold a part in slot 0
-    int64_t parts = 1;
-    for (bool more = true; more;) {
-      const int64_t q = chunk + parts + threadIdx.x;
-      const uint64_t differ =
-          __ballot(q >= ch.count || s.key[q * ch.size] != key);
-      if (lane == 0)
-        wave_end[wave] = differ ? __ffsll((long long)differ) - 1 : kWave;
-      __syncthreads();
-      for (int w = 0; more && w < kJoinBlock / kWave; w++) {
-        parts += wave_end[w];
-        more = wave_end[w] == kWave;
-      }
-      __syncthreads();
-    }
-    int64_t at = ((item % tiles) * tpr + in) * kVec;
-    if (kTiny)
-      at = 0;
-    else if (at + kVec > a.dim)
-      at = a.dim - kVec;
-    const Cols<kTiny> c(0, kTiny ? (int)a.dim : kVec);
+  const int64_t runs = *starts.count, items = runs * tiles;
+  const Cols<kTiny> c(0, kTiny ? (int)a.dim : kVec);
+  // every `of`-th of the parts from `first` on
+  auto add_parts = [&](int64_t chunk, int64_t parts, int64_t at, int first,
+                       int of) {
     constexpr int kAhead = 8;
     float8 acc = 0.f;
-    for (int64_t j = team; j < parts; j += teams * kAhead) {
+    for (int64_t j = first; j < parts; j += of * kAhead) {
       float8 part[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; i++) {
-        const int64_t k = j + i * teams;  // part 0 is in slot 1
+        const int64_t k = j + i * of;  // part 0 is in slot 1
         part[i] = 0.f;
         if (k < parts)
           part[i] =
@@ -456,15 +447,75 @@ __global__ __launch_bounds__(kJoinBlock) void embedding_join_kernel(
 #pragma unroll
       for (int i = 0; i < kAhead; i++) acc += part[i];
     }
-    *(float8*)&joint[threadIdx.x * kVec] = acc;
-    __syncthreads();
-    if (team == 0) {
-      const int used = parts < teams ? (int)parts : teams;
-      for (int t = 1; t < used; t++)
-        acc += *(const float8*)&joint[(t * tpr + in) * kVec];
-      c.store((W*)a.dweight + (int64_t)key * a.dim + at, acc * a.scale);
+    return acc;
+  };
+  for (int64_t base = (int64_t)blockIdx.x * kRuns; base < items;
+       base += (int64_t)gridDim.x * kRuns) {
+    // with kMany a run's tiles are far apart, so that no workgroup has many
+    // long ones
+    auto find = [&](int64_t item, int64_t& chunk, int32_t& key, int64_t& at) {
+      chunk = starts.chunk[kMany ? item % runs : item / tiles];
+      key = s.key[(chunk + 1) * ch.size - 1];
+      at = ((kMany ? item / runs : item % tiles) * tpr + in) * kVec;
+      if (kTiny)
+        at = 0;
+      else if (at + kVec > a.dim)
+        at = a.dim - kVec;
+    };
+    int64_t chunk, at;
+    int32_t key;
+    if constexpr (kMany) {
+      bool more = false;
+      if (base + wave < items) {
+        find(base + wave, chunk, key, at);
+        const int few = 16 * kWave / tpr < kWave ? 16 * kWave / tpr : kWave;
+        // chunks that begin with the key hold a part in slot 0
+        const int64_t q = chunk + 1 + lane;
+        const uint64_t differ =
+            __ballot(q >= ch.count || s.key[q * ch.size] != key);
+        const int parts = differ ? __ffsll((long long)differ) : kWave + 1;
+        more = parts > few;
+        if (!more) {
+          float8 acc = add_parts(chunk, parts, at, lane / tpr, kWave / tpr);
+          for (int o = tpr; o < kWave; o <<= 1)
+#pragma unroll
+            for (int i = 0; i < kVec; i++) acc[i] += __shfl_xor(acc[i], o);
+          if (lane < tpr)
+            c.store((W*)a.dweight + (int64_t)key * a.dim + at, acc * a.scale);
+        }
+      }
+      if (lane == 0) many[wave] = more;
+      __syncthreads();
     }
-    __syncthreads();
+    for (int w = 0; w < kRuns; w++) {
+      if (kMany && !many[w]) continue;
+      find(base + w, chunk, key, at);
+      int64_t parts = 1;
+      for (bool on = true; on;) {
+        const int64_t q = chunk + parts + threadIdx.x;
+        const uint64_t differ =
+            __ballot(q >= ch.count || s.key[q * ch.size] != key);
+        if (lane == 0)
+          wave_end[wave] = differ ? __ffsll((long long)differ) - 1 : kWave;
+        __syncthreads();
+        for (int v = 0; on && v < kWaves; v++) {
+          parts += wave_end[v];
+          on = wave_end[v] == kWave;
+        }
+        __syncthreads();
+      }
+      float8 acc = add_parts(chunk, parts, at, team, teams);
+      *(float8*)&joint[threadIdx.x * kVec] = acc;
+      __syncthreads();
+      if (team == 0) {
+        const int used = parts < teams ? (int)parts : teams;
+        for (int t = 1; t < used; t++)
+          acc += *(const float8*)&joint[(t * tpr + in) * kVec];
+        c.store((W*)a.dweight + (int64_t)key * a.dim + at, acc * a.scale);
+      }
+      __syncthreads();
+    }
+    if (kMany) __syncthreads();  // before `many` is written again
   }
 }
 
@@ -584,7 +635,8 @@ hipError_t embedding_backward(const EmbeddingBwd& a, hipStream_t stream) {
     // at least 4 bits: the placing reads the counts of four digits at once
     const int even = (bits + passes - 1) / passes, digit = even < 4 ? 4 : even;
     Tiles tiles;
-    tiles.size = (a.n + kMaxTiles - 1) / kMaxTiles;
+    const int64_t most = a.n < 131072 ? 64 : a.n < 524288 ? 128 : kMaxTiles;
+    tiles.size = (a.n + most - 1) / most;
     tiles.size = (tiles.size + kSortBlock - 1) / kSortBlock * kSortBlock;
     tiles.count = (a.n + tiles.size - 1) / tiles.size;
     zero.launches = 2 * passes;
@@ -601,6 +653,10 @@ hipError_t embedding_backward(const EmbeddingBwd& a, hipStream_t stream) {
   }
   if (a.n == 0) return hipGetLastError();
 
+  // at most as many runs cross borders as there are chunks or tokens to tell
+  // apart
+  const bool many_runs =
+      (ch.count < a.vocab ? ch.count : a.vocab) * ch.tiles > 8192;
   with_type(a.wtype, [&](auto* w) {
     using W = std::remove_pointer_t<decltype(w)>;
     auto sums = [&](auto tiny) {
@@ -610,9 +666,11 @@ hipError_t embedding_backward(const EmbeddingBwd& a, hipStream_t stream) {
         launch(embedding_sum_kernel<D, W, kTiny>, (uint32_t)blocks, kBlock,
                stream, a, sorted, ch, starts, partial);
       });
-      if (ch.count > 1)
-        launch(embedding_join_kernel<W, kTiny>, kJoinBlocks, kJoinBlock, stream,
-               a, sorted, ch, starts, (const float*)partial);
+      if (ch.count < 2) return;
+      const auto join = many_runs ? embedding_join_kernel<W, kTiny, true>
+                                  : embedding_join_kernel<W, kTiny, false>;
+      launch(join, kJoinBlocks, kJoinBlock, stream, a, sorted, ch, starts,
+             (const float*)partial);
     };
     if (a.dim < kVec)
       sums(std::true_type());

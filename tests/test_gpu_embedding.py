@@ -85,6 +85,19 @@ def test_long(n):
     case(3000, 16, n, wtype=F32, tok=tok, seed=n)
 
 
+@pytest.mark.parametrize("vocab,dim,n", [
+    (20000, 40, 200000), (30000, 5, 150000), (12000, 1000, 131072),
+    (9000, 2056, 70000), (20000, 17, 600000)])
+def test_many_runs(vocab, dim, n):
+    """Tokens with frequencies over their rank: some runs of thousands and
+    thousands of runs of a few."""
+    g = torch.Generator().manual_seed(dim)
+    u = torch.rand(n, generator=g, dtype=torch.float64)
+    tok = ((vocab + 1.0) ** u - 1.0).long().clamp_(0, vocab - 1)
+    case(vocab, dim, n, tok=torch.randperm(vocab, generator=g)[tok], scale=0.5,
+         pad=3, seed=n)
+
+
 @pytest.mark.parametrize("wtype", [BF, HF, F32])
 @pytest.mark.parametrize("out", [BF, HF, F32])
 def test_types(wtype, out):
