@@ -12,9 +12,9 @@
 // touch a gradient.
 //
 // 65536 tokens, a table of 131072 x 4096 bf16: lookup 151 us (7.1 TB/s read
-// and written: rows that are asked for again come from a cache), gradient 363
-// us, of which the sort with the zeroing of dW (1.07 GB) beside it takes 172,
-// the sums 177 and the join of runs 14.  A large copy moves 5.0 TB/s, a fill
+// and written: rows that are asked for again come from a cache), gradient 368
+// us, of which the sort with the zeroing of dW (1.07 GB) beside it takes 175,
+// the sums 179 and the join of runs 14.  A large copy moves 5.0 TB/s, a fill
 // 6.8.
 #include <hip/hip_runtime.h>
 
