@@ -55,6 +55,8 @@ void check_act(const Tensor& t, const char* op, const char* name) {
   TORCH_CHECK(t.layout() == at::kStrided, op, ": ", name, " must be dense");
   TORCH_CHECK(is_act_type(t.scalar_type()), op, ": ", name,
               " must be float32, bfloat16 or float16, not ", t.scalar_type());
+  TORCH_CHECK(!t.is_neg(), op, ": ", name,
+              " is a view that stands for its negative; resolve_neg() it");
 }
 
 void check_device(const Tensor& t, const Tensor& on, const char* op,
@@ -66,7 +68,10 @@ void check_device(const Tensor& t, const Tensor& on, const char* op,
 
 // Whether a gradient will be asked of any of these.  Without one an operator
 // runs alone, keeps nothing and makes no graph.
-bool wants_grad(std::initializer_list<const Tensor*> tensors) {
+bool wants_grad(const char* op, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(), op,
+                ": no forward-mode gradient");
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : tensors)
     if (t && t->defined() && t->requires_grad()) return true;
@@ -120,7 +125,8 @@ struct Rows {
   int64_t stride;
 };
 
-Rows as_rows(const Tensor& t) {
+Rows as_rows(const Tensor& given) {
+  const Tensor t = given.resolve_neg();
   const int64_t dim = t.size(-1);
   bool ok = dim <= 1 || t.stride(-1) == 1;
   int64_t stride = dim, next = -1;
@@ -232,7 +238,7 @@ Tensor embedding(const Tensor& weight, const Tensor& tokens, double scale,
   check_device(weight, weight, op, "weight");
   check_device(tokens, weight, op, "tokens");
   const Tensor tok = tokens.contiguous();
-  if (!wants_grad({&weight})) return lookup(weight, tok, scale, out);
+  if (!wants_grad(op, {&weight})) return lookup(weight, tok, scale, out);
   const auto node = make_node<EmbeddingNode>(weight);
   node->vocab = vocab;
   node->padding = padding;
@@ -456,7 +462,7 @@ Tensor rms_norm(const Tensor& x, const OptTensor& weight, double eps) {
   if (weight) check_device(*weight, x, op, "weight");
   const NormArgs n = {x,   {},  {},  {},          contiguous(weight), 1.0,
                       1.0, eps, Gate::kNone, 1, true};
-  return std::get<1>(wants_grad({&x, &n.pre}) ? norm_with_grad(n)
+  return std::get<1>(wants_grad(op, {&x, &n.pre}) ? norm_with_grad(n)
                                               : run_norm(n, Tensor()));
 }
 
@@ -531,7 +537,7 @@ std::tuple<Tensor, OptTensor> gated_residual_norm(
                       mode,
                       group_rows,
                       pre_weight.has_value()};
-  auto [y, h] = wants_grad({&x, &branch, &g, &n.post, &n.pre})
+  auto [y, h] = wants_grad(op, {&x, &branch, &g, &n.post, &n.pre})
                     ? norm_with_grad(n)
                     : run_norm(n, Tensor());
   return {y, n.want_h ? OptTensor(h) : OptTensor()};
@@ -772,7 +778,7 @@ Tensor linear_act8(const Tensor& x, const Tensor& weight,
   const c10::impl::ExcludeDispatchKeyGuard own_types(
       c10::autocast_dispatch_keyset);
   const c10::OptionalDeviceGuard guard(x.device());
-  if (!wants_grad({&x, &weight, get(bias)}))
+  if (!wants_grad(op, {&x, &weight, get(bias)}))
     return flat_linear(x, weight, bias);
   const auto node = make_node<LinearAct8Node>(x, weight, bias);
   node->k = x.size(-1);
@@ -845,7 +851,7 @@ Tensor silu_mul_act8(const Tensor& x) {
               ": x must hold two halves in its last dimension, not ",
               x.size(-1), " columns");
   check_device(x, x, op, "x");
-  if (!wants_grad({&x})) return run_silu(x, Tensor(), Tensor());
+  if (!wants_grad(op, {&x})) return run_silu(x, Tensor(), Tensor());
   const auto node = make_node<SiluAct8Node>(x);
   const at::NoGradGuard no_grad;
   const c10::OptionalDeviceGuard guard(x.device());

@@ -332,3 +332,28 @@ def test_kept_tensors_are_guarded():
     x.mul_(2.0)
     with pytest.raises(RuntimeError, match="inplace"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_forward_mode_is_refused(which):
+    from torch.autograd import forward_ad
+
+    f, leaves = _each_operator()[which]
+    for i, leaf in enumerate(leaves):
+        with forward_ad.dual_level(), torch.no_grad():
+            duals = [t.detach() for t in leaves]
+            duals[i] = forward_ad.make_dual(duals[i], torch.ones_like(leaf))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f(*duals)
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_gradient_as_a_negated_view(which):
+    f, leaves = _each_operator()[which]
+    y = f(*leaves)
+    dout = torch.randn_like(y)
+    want = torch.autograd.grad(y, leaves, -dout, retain_graph=True,
+                               allow_unused=True)
+    got = torch.autograd.grad(y, leaves, torch._neg_view(dout),
+                              allow_unused=True)
+    assert all(a is b or torch.equal(a, b) for a, b in zip(got, want))

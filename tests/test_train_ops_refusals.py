@@ -32,6 +32,8 @@ TOK = torch.zeros(3, dtype=torch.int64)
     (lambda: ops.rms_norm(_bf(2, 16385)), "at most 16384 columns"),
     (lambda: ops.rms_norm(_bf(4, 8), eps=-1.0), "eps"),
     (lambda: ops.rms_norm(_bf(4, 8)), "x must be on the GPU"),
+    (lambda: ops.rms_norm(torch._neg_view(_bf(4, 8))), "resolve_neg"),
+    (lambda: ops.embedding(torch._neg_view(_bf(4, 8)), TOK), "resolve_neg"),
     (lambda: ops.gated_residual_norm(_bf(4, 8), _bf(4, 9)), "x's shape"),
     (lambda: ops.gated_residual_norm(_bf(4, 8), torch.zeros(4, 8)),
      "x's type"),
