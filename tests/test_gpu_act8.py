@@ -161,6 +161,29 @@ def test_wgrad_of_uneven_sizes(dtype, m, n, k):
     wgrad(m, n, k, dtype, seed=n)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("m,n,k", [
+    (1, 3, 40), (2, 1, 33), (63, 7, 8), (64, 255, 64), (65, 257, 300),
+    (129, 9, 500), (4097, 129, 40), (640, 513, 1025), (900, 4353, 4000)])
+def test_wgrad_of_odd_rows(dtype, m, n, k):
+    """The last value of dy lies in half of the 4 bytes that reads count."""
+    wgrad(m, n, k, dtype, seed=m)
+    from baguanet import ops
+
+    # that value alone, exact, from a tensor that ends with its storage and
+    # from the middle of a larger one
+    for dy in (torch.zeros(m, n, dtype=dtype, device="cuda"),
+               torch.full((m + 2, n + 4), 7.0, dtype=dtype,
+                          device="cuda")[1:m + 1, 3:n + 3]):
+        dy.zero_()
+        dy[-1, -1] = 3.0
+        x = rows((m, k), dtype, 3).cuda()
+        dw, db = ops.act8_wgrad(dy, ops.act8_pack(x))
+        want = kept(x)[-1].cuda() * 3.0
+        assert torch.equal(dw[-1], want.to(dtype))
+        assert (dw[:-1] == 0).all() and (db[:-1] == 0).all() and db[-1] == 3
+
+
 def test_wgrad_strides():
     big = rows((200, 150), BF, 3, wild=False).cuda()
     for dy in (big[:, 3:77], big[::2, 1:], big.t(), big[:1].expand(90, 150),
