@@ -58,13 +58,13 @@ __device__ inline void row_sums(float (&v)[N], float* red) {
 
 template <int TPR>
 constexpr int block_of() {
-  return TPR < 256 ? 256 : TPR;
+  return TPR <= kWave ? 256 : TPR;
 }
 
 // The team of a thread: its wave where that is a team, as a uniform number.
 template <int TPR>
 __device__ inline int team_of() {
-  if constexpr (TPR >= 256) return 0;
+  if constexpr (TPR > kWave) return 0;
   return __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
 }
 
@@ -163,11 +163,13 @@ struct Parts {
   float *pre, *post, *group;
 };
 
-// kSeam: the whole seam (branch with its norm, both gradients, a gate of
-// groups or none), as every block of a network but the first has it.  Left to
-// the arguments, these choices cost about 60 registers and with them half of
-// the waves in flight.
-template <typename T, int TPR, int VPT, bool kTiny, bool kSeam>
+// kWhole: the whole seam (branch with its norm, both gradients, a gate of
+// groups or none), as every block of a network but the first has it; kRows:
+// the same with a gate for each row.  Left to the arguments, these choices cost
+// registers, and with them waves in flight, and tests at each use.
+enum class Seam { kAny, kWhole, kRows };
+
+template <typename T, int TPR, int VPT, bool kTiny, Seam kind>
 __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
     NormBwd a, Cut cut, Parts parts) {
   constexpr int kTeams = block_of<TPR>() / TPR;
@@ -178,12 +180,15 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
   // wide rows: sums over rows that registers have no room for, for each lane
   constexpr bool kWide = TPR * VPT > 1024;
   __shared__ float held[kWide ? 2 * TPR * VPT * kVec : 1];
+  constexpr bool kSeam = kind != Seam::kAny;
   const bool has_branch = kSeam || a.branch, has_post = kSeam || a.post;
   const bool has_dy = kSeam || a.dy, has_dh = kSeam || a.dh;
-  const Gate gmode = kSeam && a.gmode != Gate::kNone ? Gate::kGroup : a.gmode;
-  const bool full = !kSeam && gmode == Gate::kFull;
-  const bool per_row = !kSeam && gmode == Gate::kRow;
-  const bool grouped = gmode == Gate::kGroup;
+  const bool full = !kSeam && a.gmode == Gate::kFull;
+  const bool per_row =
+      kind == Seam::kRows || (!kSeam && a.gmode == Gate::kRow);
+  const bool grouped =
+      kind != Seam::kRows &&
+      (kSeam ? a.gmode != Gate::kNone : a.gmode == Gate::kGroup);
   const bool one_gate = grouped && cut.groups == 1;
   const int lane = threadIdx.x % TPR, team = team_of<TPR>();
   const float inv_dim = 1.f / (float)a.dim;
@@ -463,19 +468,20 @@ __global__ __launch_bounds__(kJoinCols* kJoinStrips) void norm_join_kernel(
   }
 }
 
-constexpr int64_t kTargetBlocks = 512;
-
 Cut cut_rows(const NormBwd& a) {
   Cut c;
+  // 2048 waves at work, or more where a row takes more than four
+  const bool pairs = a.dim > 512 && a.dim <= 1024 && a.type != ElemType::kF32;
+  const int64_t target = pairs ? 1024 : 512;
   const bool grouped = a.gmode == Gate::kGroup && a.branch;
   c.group_rows = grouped ? a.group_rows : a.rows;
   c.groups = a.rows / c.group_rows;
-  if (c.groups >= kTargetBlocks) {
-    c.per_block = (c.groups + kTargetBlocks - 1) / kTargetBlocks;
+  if (c.groups >= target) {
+    c.per_block = (c.groups + target - 1) / target;
     c.slices = 1;
   } else {
     c.per_block = 1;
-    c.slices = kTargetBlocks / c.groups;
+    c.slices = target / c.groups;
     // at least 8 rows for a workgroup, or its parts cost more than the rows
     const int64_t most = (c.group_rows + 7) / 8;
     if (c.slices > most) c.slices = most;
@@ -497,7 +503,11 @@ bool wants_group(const NormBwd& a, const Cut& c) {
 }
 
 // Calls f with the team size and vectors per lane that hold `dim` columns.
-template <typename F>
+// kPairs: up to 1024 columns two waves share a row rather than one taking two
+// vectors a lane.  That is for 2-byte gradients: 60000 rows of 787 bf16 take
+// 139 us so and 160 with one wave, of 1000 fp32 307 and 299; the forward pass
+// takes 90 and 77.
+template <bool kPairs, typename F>
 void with_team(int64_t dim, F&& f) {
   if (dim < kVec)
     f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>(),
@@ -506,8 +516,8 @@ void with_team(int64_t dim, F&& f) {
     f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>(),
       std::false_type());
   else if (dim <= 1024)
-    f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>(),
-      std::false_type());
+    f(std::integral_constant<int, kPairs ? 128 : 64>(),
+      std::integral_constant<int, kPairs ? 1 : 2>(), std::false_type());
   else if (dim <= 2048)
     f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>(),
       std::false_type());
@@ -529,7 +539,7 @@ hipError_t norm_forward(const NormFwd& a, hipStream_t stream) {
   if (a.dim > kNormMaxDim) return hipErrorInvalidValue;
   with_type(a.type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    with_team(a.dim, [&](auto tpr, auto vpt, auto tiny) {
+    with_team<false>(a.dim, [&](auto tpr, auto vpt, auto tiny) {
       constexpr int kTpr = decltype(tpr)::value, kVpt = decltype(vpt)::value;
       constexpr bool kTiny = decltype(tiny)::value;
       constexpr int kBlk = block_of<kTpr>();
@@ -563,17 +573,17 @@ hipError_t norm_backward(const NormBwd& a, hipStream_t stream) {
   if (wants_group(a, c)) parts.group = ws, ws += part;
   with_type(a.type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    with_team(a.dim, [&](auto tpr, auto vpt, auto tiny) {
+    with_team<sizeof(T) == 2>(a.dim, [&](auto tpr, auto vpt, auto tiny) {
       constexpr int kTpr = decltype(tpr)::value, kVpt = decltype(vpt)::value;
       constexpr bool kTiny = decltype(tiny)::value;
-      const bool seam = a.branch && a.post && a.dy && a.dh &&
-                        (a.gmode == Gate::kNone || a.gmode == Gate::kGroup);
-      if (seam)
-        launch(norm_backward_kernel<T, kTpr, kVpt, kTiny, true>,
-               (uint32_t)c.blocks, block_of<kTpr>(), stream, a, c, parts);
-      else
-        launch(norm_backward_kernel<T, kTpr, kVpt, kTiny, false>,
-               (uint32_t)c.blocks, block_of<kTpr>(), stream, a, c, parts);
+      const bool whole = a.branch && a.post && a.dy && a.dh;
+      const auto kernel =
+          !whole || a.gmode == Gate::kFull
+              ? norm_backward_kernel<T, kTpr, kVpt, kTiny, Seam::kAny>
+          : a.gmode == Gate::kRow
+              ? norm_backward_kernel<T, kTpr, kVpt, kTiny, Seam::kRows>
+              : norm_backward_kernel<T, kTpr, kVpt, kTiny, Seam::kWhole>;
+      launch(kernel, (uint32_t)c.blocks, block_of<kTpr>(), stream, a, c, parts);
     });
     if (parts.pre || parts.post || parts.group) {
       const dim3 grid((uint32_t)((a.dim + kJoinCols - 1) / kJoinCols),
