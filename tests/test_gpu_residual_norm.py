@@ -175,6 +175,23 @@ def test_groups(shape, gate):
     case(shape, gate=gate, bs=0.5)
 
 
+@pytest.mark.parametrize("kind", ["none", "column", "group", "row", "each"])
+@pytest.mark.parametrize("dim", [3, 300, 600, 787, 1024, 1999, 4000, 8000,
+                                 9001])
+def test_gates_of_every_width(kind, dim):
+    gate = {"none": None, "column": (dim,), "group": (3, 1, dim),
+            "row": (3, 37, 1), "each": (3, 37, dim)}[kind]
+    case((3, 37, dim), dtype=HF if dim % 2 else BF, gate=gate, bs=0.5,
+         seed=dim)
+
+
+@pytest.mark.parametrize("shape,gate", [
+    ((1100, 2, 787), (1100, 1, 787)), ((2, 1500, 787), (2, 1, 787)),
+    ((4099, 600), (4099, 1)), ((9000, 1000), None)])
+def test_rows_of_two_waves(shape, gate):
+    case(shape, gate=gate, bs=0.5)
+
+
 @pytest.mark.parametrize("use", [("y",), ("h",)])
 @pytest.mark.parametrize("post", [True, False])
 def test_one_output_used(use, post):
