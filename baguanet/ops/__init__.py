@@ -113,7 +113,9 @@ def fused_sgd(params, grads, momenta, lr, momentum=0.0, weight_decay=0.0,
 # ---------------------------------------------------------------------------
 # Training-step operators.  Each takes float32, bfloat16 or float16 tensors on
 # the GPU, runs on the current stream, sums in float32 and rounds once; each
-# is differentiable once, with the same result in every run.
+# is differentiable once, with the same result in every run.  Calls may be
+# captured into a graph; a backward pass only while no eager graph of the same
+# leaves is alive, as with torch's own operators.
 
 
 def embedding(weight: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
