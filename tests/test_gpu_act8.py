@@ -78,6 +78,26 @@ def test_kept_values(dtype, shape):
     assert got.dtype == dtype and same(got, kept(x))
 
 
+@pytest.mark.parametrize("shape", [(1, 2048), (1, 2049), (2, 4096), (3, 4129),
+                                   (511, 2081), (512, 2081), (4, 70000)])
+def test_rows_in_pieces(shape):
+    """Few long rows are cut: whole, and beside the gated activation."""
+    from baguanet import ops
+
+    x = rows(shape, BF, 7)
+    assert same(ops.act8_unpack(ops.act8_pack(x.cuda())), kept(x))
+    both = torch.cat([x, x.flip(-1)], -1).cuda().requires_grad_()
+    out = ops.silu_mul_act8(both)
+    g = torch.ones_like(out)
+    (dx,) = torch.autograd.grad(out, both, g)
+    for r in (0, shape[0] - 1):  # a row comes out as it does alone
+        one = both.detach()[r:r + 1].clone().requires_grad_()
+        few = ops.silu_mul_act8(one)
+        assert torch.equal(out[r:r + 1], few)
+        assert torch.equal(dx[r:r + 1],
+                           torch.autograd.grad(few, one, g[r:r + 1])[0])
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
 def test_every_magnitude(dtype):
     """From the smallest to the largest numbers of the type, ties among
