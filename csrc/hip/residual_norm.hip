@@ -338,7 +338,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
       const float sq = s[1] - k0 * s[2];
       const float k1 = sq * g_row * inv_dim;
       if (per_row && a.dgate && lane == 0) {
-        if (a.gate32)
+        if (a.dgate32)
           ((float*)a.dgate)[row] = sq;
         else
           ((T*)a.dgate)[row] = (T)sq;
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
           if (full) {
             const float8 g = gate_at(j, row * a.dim);
             if (a.dgate && c[j].own())
-              c[j].template put_weight<T>(a.dgate, a.gate32, row * a.dim,
+              c[j].template put_weight<T>(a.dgate, a.dgate32, row * a.dim,
                                           e * k);
             e *= g;
             du *= g;
@@ -376,7 +376,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
           if (!c[j].own()) continue;
           if (a.dgate && cut.slices == 1)
             c[j].template put_weight<T>(
-                a.dgate, a.gate32, grp * a.dim,
+                a.dgate, a.dgate32, grp * a.dim,
                 acc_post[j] * post_at(j) * a.branch_scale);
           if (parts.group)
             c[j].store(parts.group + blockIdx.x * a.dim, acc_post[j]);
@@ -457,15 +457,88 @@ __global__ __launch_bounds__(kJoinCols* kJoinStrips) void norm_join_kernel(
     sum *= a.branch_scale;
     if (a.gmode == Gate::kGroup && cut.groups == 1) {
       if (a.dgate)
-        put(a.dgate, a.gate32, col,
+        put(a.dgate, a.dgate32, col,
             sum * (a.post ? get(a.post, a.post32) : 1.f));
       sum *= get(a.gate, a.gate32);
     }
     if (a.dpost) put(a.dpost, a.post32, col, sum);
   } else {
     sum *= a.branch_scale * (a.post ? get(a.post, a.post32) : 1.f);
-    put(a.dgate, a.gate32, (what - 2) * a.dim + col, sum);
+    put(a.dgate, a.dgate32, (what - 2) * a.dim + col, sum);
   }
+}
+
+// out[o, i] = the sum of in[o, r, i] over r, in fp32 and in a fixed order.  A
+// team of `cols` by `strips` threads (powers of two) takes `cols` neighbours
+// of i; its strips take every so many of the rows of blockIdx.y's slice, and
+// their sums are added in pairs.  Bound by HBM: each value is read once.
+constexpr int kGateBlock = 256;
+
+struct GateCut {
+  int cols, strips;
+  int64_t tiles, items;  // of i for one o, and in all
+  int64_t slices, slice_rows;
+};
+
+template <typename O>
+__global__ __launch_bounds__(kGateBlock) void norm_gate_kernel(GateSum a,
+                                                               GateCut g,
+                                                               O* out) {
+  __shared__ float sums[kGateBlock];
+  const int team = g.cols * g.strips, teams = kGateBlock / team;
+  const int in = threadIdx.x % team, strip = in / g.cols;
+  const int64_t r0 = blockIdx.y * g.slice_rows;
+  const int64_t r1 = r0 + g.slice_rows < a.rows ? r0 + g.slice_rows : a.rows;
+  for (int64_t first = (int64_t)blockIdx.x * teams; first < g.items;
+       first += (int64_t)gridDim.x * teams) {
+    const int64_t item = first + threadIdx.x / team;
+    const int64_t o = item / g.tiles;
+    const int64_t i = item % g.tiles * g.cols + in % g.cols;
+    const bool live = item < g.items && i < a.inner;
+    float sum = 0.f;
+    if (live) {
+      const float* p = a.in + o * a.rows * a.inner + i;
+#pragma unroll 4
+      for (int64_t r = r0 + strip; r < r1; r += g.strips)
+        sum += p[r * a.inner];
+    }
+    for (int half = g.strips / 2; half; half /= 2) {
+      __syncthreads();
+      sums[threadIdx.x] = sum;
+      __syncthreads();
+      if (strip < half) sum += sums[threadIdx.x + half * g.cols];
+    }
+    if (live && strip == 0)
+      out[(o * g.slices + blockIdx.y) * a.inner + i] = (O)sum;
+  }
+}
+
+// Slices of the rows where one workgroup for each tile would leave compute
+// units idle; a second launch adds the slices' sums.
+GateCut cut_gate(const GateSum& a) {
+  GateCut g = {1, 1, 1, 0, 1, a.rows};
+  while (g.cols < kWave && g.cols < a.inner) g.cols *= 2;
+  while (g.cols * g.strips < kGateBlock && g.strips < a.rows) g.strips *= 2;
+  g.tiles = (a.inner + g.cols - 1) / g.cols;
+  g.items = a.outer * g.tiles;
+  const int64_t teams = kGateBlock / (g.cols * g.strips);
+  const int64_t blocks = (g.items + teams - 1) / teams;
+  const int64_t most = (a.rows + g.strips * 16 - 1) / (g.strips * 16);
+  const int64_t want = 1024 / (blocks < 1024 ? blocks : 1024);
+  g.slices = most < want ? most : want;
+  g.slice_rows = (a.rows + g.slices - 1) / g.slices;
+  g.slices = (a.rows + g.slice_rows - 1) / g.slice_rows;
+  return g;
+}
+
+template <typename O>
+void launch_gate(const GateSum& a, const GateCut& g, O* out,
+                 hipStream_t stream) {
+  const int64_t teams = kGateBlock / (g.cols * g.strips);
+  const int64_t blocks = (g.items + teams - 1) / teams;
+  launch(norm_gate_kernel<O>,
+         dim3((uint32_t)(blocks < 65536 ? blocks : 65536), (uint32_t)g.slices),
+         kGateBlock, stream, a, g, out);
 }
 
 Cut cut_rows(const NormBwd& a) {
@@ -591,6 +664,32 @@ hipError_t norm_backward(const NormBwd& a, hipStream_t stream) {
       launch(norm_join_kernel<T>, grid, kJoinCols * kJoinStrips, stream, a, c,
              parts);
     }
+  });
+  return hipGetLastError();
+}
+
+size_t norm_gate_workspace(const GateSum& a) {
+  if (a.outer == 0 || a.rows == 0 || a.inner == 0) return 0;
+  const GateCut g = cut_gate(a);
+  return g.slices > 1 ? (size_t)(a.outer * g.slices * a.inner) * sizeof(float)
+                      : 0;
+}
+
+hipError_t norm_gate_sum(const GateSum& a, hipStream_t stream) {
+  if (a.outer == 0 || a.rows == 0 || a.inner == 0) return hipSuccess;
+  GateSum last = a;
+  GateCut g = cut_gate(a);
+  if (g.slices > 1) {
+    launch_gate(a, g, a.workspace, stream);
+    last.in = a.workspace;
+    last.rows = g.slices;
+    g = cut_gate(last);
+    g.slices = 1;
+    g.slice_rows = last.rows;
+  }
+  with_type(a.type, [&](auto* t) {
+    using O = std::remove_pointer_t<decltype(t)>;
+    launch_gate(last, g, (O*)a.out, stream);
   });
   return hipGetLastError();
 }

@@ -78,7 +78,7 @@ struct NormBwd {
   const float* ry;
   void* dx;            // [rows, dim]
   void* dbranch;       // [rows, dim] (with a branch)
-  void* dgate;         // the gate's shape, or null
+  void* dgate;         // the gate's shape, or null; fp32 if dgate32, else T
   void* dpost;         // [dim], or null
   void* dpre;          // [dim], or null
   void* workspace;     // norm_workspace() bytes
@@ -86,11 +86,23 @@ struct NormBwd {
   int64_t group_rows;
   float residual_scale, branch_scale;
   Gate gmode;
-  bool gate32, post32, pre32;
+  bool gate32, post32, pre32, dgate32;
   ElemType type;
 };
 size_t norm_workspace(const NormBwd& a);
 hipError_t norm_backward(const NormBwd& a, hipStream_t stream);
+
+// The gradient of a gate that is repeated: the sum of [outer, rows, inner]
+// over its rows.
+struct GateSum {
+  const float* in;     // [outer, rows, inner]
+  void* out;           // [outer, inner]
+  float* workspace;    // norm_gate_workspace() bytes
+  int64_t outer, rows, inner;
+  ElemType type;       // of out
+};
+size_t norm_gate_workspace(const GateSum& a);
+hipError_t norm_gate_sum(const GateSum& a, hipStream_t stream);
 
 // ---- 8-bit activation checkpoints (act8.hip, act8_wgrad.hip) ---------------
 

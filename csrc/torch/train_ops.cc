@@ -254,13 +254,68 @@ Tensor embedding(const Tensor& weight, const Tensor& tokens, double scale,
 // ---------------------------------------------------------------------------
 // gated residual norm
 
+// What a gate's gradient is summed over: the kernels give one value for each
+// row or element, and the gate has fewer.  In fp32, so that it is rounded once.
+struct Repeated {
+  std::vector<int64_t> sizes;  // of the kernels' gate, or empty: as it is
+  int64_t outer, rows, inner;  // the sizes merged, `rows` to be summed
+  // several dimensions apart from each other: the others first, then those
+  std::vector<int64_t> order;
+};
+
 struct NormArgs {
   Tensor x, branch, gate, post, pre;  // undefined where not given
   double residual_scale, branch_scale, eps;
   Gate gmode;
   int64_t group_rows;
   bool want_h;
+  Tensor gate_leaf;  // as it was given: it takes the gradient
+  Repeated repeated;
 };
+
+// A gate of the sizes `own` in the place of one of `to`, with as many
+// dimensions (leading ones of 1 stand for those that it lacks).
+Repeated repeated_over(const std::vector<int64_t>& own,
+                       const std::vector<int64_t>& to) {
+  Repeated r = {};
+  if (own == to) return r;
+  r.sizes = to;
+  r.outer = r.rows = r.inner = 1;
+  bool split = false;  // an own dimension between two repeated ones
+  for (size_t d = 0; d < to.size(); d++) {
+    if (to[d] == 1) continue;
+    if (own[d] == to[d]) {
+      (r.rows == 1 ? r.outer : r.inner) *= to[d];
+    } else {
+      split |= r.inner != 1;
+      r.rows *= to[d];
+    }
+  }
+  if (!split) return r;
+  for (const bool repeat : {false, true})
+    for (size_t d = 0; d < to.size(); d++)
+      if ((own[d] != to[d]) == repeat) r.order.push_back((int64_t)d);
+  r.outer *= r.inner;
+  r.inner = 1;
+  return r;
+}
+
+// The gate's gradient from that of each row or element.
+Tensor sum_repeated(const Repeated& r, const Tensor& each, const Tensor& out) {
+  const Tensor in = r.order.empty() ? each : each.permute(r.order).contiguous();
+  GateSum a = {};
+  a.in = in.data_ptr<float>();
+  a.out = out.data_ptr();
+  a.outer = r.outer;
+  a.rows = r.rows;
+  a.inner = r.inner;
+  a.type = elem(out.scalar_type());
+  if (in.numel() == 0) out.zero_();
+  const Tensor ws = empty_bytes(norm_gate_workspace(a), in);
+  a.workspace = (float*)ws.data_ptr();
+  check_launch(norm_gate_sum(a, stream_of(in)), "residual norm backward");
+  return out;
+}
 
 // y (where there is a branch) and h (where it is wanted); `stats`: [2, rows],
 // the reciprocals that the backward pass takes, or undefined.
@@ -314,6 +369,8 @@ struct NormNode : OpNode<6> {
   double residual_scale, branch_scale;
   Gate gmode;
   int64_t group_rows;
+  std::vector<int64_t> gate_sizes;
+  Repeated repeated;
 
   std::string name() const override { return "GatedResidualNormBackward"; }
 
@@ -345,6 +402,7 @@ struct NormNode : OpNode<6> {
     Tensor dx = at::empty(some.sizes(), some.options());
     a.dx = dx.data_ptr();
     Tensor dbranch, dgate, dpost, dpre;
+    Tensor each;  // dgate, before its sum over what it is repeated over
     if (dy.defined()) {
       dyr = as_rows(dy);
       a.dy = dyr.t.data_ptr();
@@ -377,8 +435,12 @@ struct NormNode : OpNode<6> {
         a.gate = gate.data_ptr();
         a.gate32 = gate.scalar_type() == at::kFloat;
         if (task_should_compute_output(2)) {
-          dgate = at::empty(gate.sizes(), gate.options());
-          a.dgate = dgate.data_ptr();
+          dgate = at::empty(gate_sizes, gate.options());
+          each = dgate;
+          if (!repeated.sizes.empty())
+            each = at::empty(repeated.sizes, gate.options().dtype(at::kFloat));
+          a.dgate = each.data_ptr();
+          a.dgate32 = each.scalar_type() == at::kFloat;
         }
       }
       if (post.defined()) {
@@ -392,12 +454,14 @@ struct NormNode : OpNode<6> {
       }
     }
     if (a.rows == 0 || a.dim == 0) {
-      for (Tensor* t : {&dgate, &dpost, &dpre})
+      for (Tensor* t : {&each, &dpost, &dpre})
         if (t->defined()) t->zero_();
     }
     const Tensor ws = empty_bytes(norm_workspace(a), dx);
     a.workspace = ws.data_ptr();
     check_launch(norm_backward(a, stream_of(dx)), "residual norm backward");
+    if (each.defined() && !repeated.sizes.empty())
+      sum_repeated(repeated, each, dgate);
     out[0] = dx;
     out[1] = dbranch;
     out[2] = dgate;
@@ -409,11 +473,14 @@ struct NormNode : OpNode<6> {
 
 // y and h as run_norm gives them, with their place in the graph.
 std::tuple<Tensor, Tensor> norm_with_grad(const NormArgs& n) {
-  const auto node = make_node<NormNode>(n.x, n.branch, n.gate, n.post, n.pre);
+  const auto node = make_node<NormNode>(n.x, n.branch, n.gate_leaf, n.post,
+                                       n.pre);
   node->residual_scale = n.residual_scale;
   node->branch_scale = n.branch_scale;
   node->gmode = n.gmode;
   node->group_rows = n.group_rows;
+  if (n.gate_leaf.defined()) node->gate_sizes = n.gate_leaf.sizes().vec();
+  node->repeated = n.repeated;
   const at::NoGradGuard no_grad;
   const Tensor stats =
       at::empty({2, rows_of(n.x)}, n.x.options().dtype(at::kFloat));
@@ -460,8 +527,9 @@ Tensor rms_norm(const Tensor& x, const OptTensor& weight, double eps) {
   TORCH_CHECK(eps >= 0, op, ": eps must not be negative");
   check_device(x, x, op, "x");
   if (weight) check_device(*weight, x, op, "weight");
-  const NormArgs n = {x,   {},  {},  {},          contiguous(weight), 1.0,
-                      1.0, eps, Gate::kNone, 1, true};
+  const NormArgs n = {x,   {},  {},          {}, contiguous(weight), 1.0,
+                      1.0, eps, Gate::kNone, 1,  true,               {},
+                      {}};
   return std::get<1>(wants_grad(op, {&x, &n.pre}) ? norm_with_grad(n)
                                               : run_norm(n, Tensor()));
 }
@@ -485,7 +553,9 @@ std::tuple<Tensor, OptTensor> gated_residual_norm(
   Gate mode = Gate::kNone;
   int64_t group_rows = rows > 0 ? rows : 1;
   Tensor g;
+  Repeated repeated = {};
   if (gate) {
+    const at::NoGradGuard no_grad;  // its gradient comes from the node
     check_act(*gate, op, "gate");
     TORCH_CHECK(gate->scalar_type() == at::kFloat ||
                     gate->scalar_type() == x.scalar_type(),
@@ -512,11 +582,12 @@ std::tuple<Tensor, OptTensor> gated_residual_norm(
       mode = group_rows == 1 && rows > 1 ? Gate::kFull : Gate::kGroup;
       if (group_rows == 0) group_rows = 1;
     } else {
-      // one value for each row, or any other pattern element by element;
-      // autograd sums the gradient back over what is repeated here
+      // one value for each row, or any other pattern element by element
       auto to = x.sizes().vec();
       mode = wide ? Gate::kFull : Gate::kRow;
       if (!wide) to.back() = 1;
+      lead.push_back(to.back());
+      repeated = repeated_over(lead, to);
       t = t.expand(to);
     }
     g = t.contiguous();
@@ -536,8 +607,10 @@ std::tuple<Tensor, OptTensor> gated_residual_norm(
                       eps,
                       mode,
                       group_rows,
-                      pre_weight.has_value()};
-  auto [y, h] = wants_grad(op, {&x, &branch, &g, &n.post, &n.pre})
+                      pre_weight.has_value(),
+                      gate ? *gate : Tensor(),
+                      repeated};
+  auto [y, h] = wants_grad(op, {&x, &branch, get(gate), &n.post, &n.pre})
                     ? norm_with_grad(n)
                     : run_norm(n, Tensor());
   return {y, n.want_h ? OptTensor(h) : OptTensor()};

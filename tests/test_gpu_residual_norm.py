@@ -419,3 +419,73 @@ def test_other_stream_and_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("shape,gate", [
+    ((6, 23, 40), g) for g in (
+        (40,), (6, 1, 40), (6, 23, 40), (6, 23, 1), (1, 23, 40), (23, 40),
+        (23, 1), (6, 1, 1), (1,), (), (1, 23, 1), (1, 1, 1))
+] + [
+    ((3, 5, 7, 40), g) for g in (
+        (5, 1, 40), (3, 1, 7, 40), (3, 1, 7, 1), (5, 1, 1), (1, 5, 1, 1),
+        (7, 1), (7, 40), (3, 1, 1, 1), (1, 5, 7, 1))
+] + [
+    ((2, 3, 4, 5, 24), g) for g in (
+        (3, 1, 5, 1), (2, 1, 4, 1, 1), (1, 3, 1, 5, 24), (2, 1, 4, 1, 24))
+] + [
+    ((1, 23, 40), (23, 1)), ((40,), (1,)), ((40,), ()), ((1, 1, 1), ()),
+    ((4, 0, 8), (4, 1, 1)), ((6, 0, 8), ()), ((4, 0, 8), (0, 8)),
+    ((20001, 24), ()), ((2, 6000, 72), (6000, 1)), ((300, 90, 16), (90, 16)),
+    ((3, 4000, 8), (3, 1, 1)), ((700, 40, 9), (700, 1, 1)),
+    ((64, 65, 264), (1, 264)), ((5000, 3, 8), (3, 1)),
+])
+def test_repeated_gates_round_once(dtype, shape, gate):
+    """A gate of two bytes that is repeated over rows or elements: its
+    gradient is summed in fp32, whatever it is repeated over."""
+    case(shape, gate=gate, dtype=dtype, wtype=dtype, bs=0.3, seed=len(gate))
+
+
+@pytest.mark.parametrize("gate", [(), (1,), (1, 1)])
+def test_repeated_gate_whose_terms_pass_its_largest(gate):
+    """Two rows give 70000 and -69000, each past fp16's 65504: their sum is
+    1000, exact in fp32 and fp16."""
+    from baguanet import ops
+
+    half = lambda v: torch.tensor(v, dtype=HF, device="cuda")
+    x, g = half([[0.0], [0.0]]), torch.ones(gate, dtype=HF, device="cuda")
+    o = half([[250.0], [250.0]])
+    g.requires_grad_()
+    y, _ = ops.gated_residual_norm(x, o, g)
+    (dg,) = torch.autograd.grad(y, g, half([[280.0], [-276.0]]))
+    assert dg.shape == g.shape and dg.item() == 1000.0
+
+
+@pytest.mark.parametrize("gate", [(), (900, 1), (900, 520), (3, 1, 1)])
+def test_repeated_gates_in_a_graph(gate):
+    """The same in every run, and in every replay of a captured pass."""
+    from baguanet import ops
+
+    rand = lambda *s: torch.randn(s, device="cuda").to(BF)
+    x, o = (rand(3, 900, 520).requires_grad_() for _ in range(2))
+    g, w = rand(*gate).requires_grad_(), rand(520).requires_grad_()
+    dy, dh = rand(3, 900, 520), rand(3, 900, 520)
+
+    def step():
+        y, h = ops.gated_residual_norm(x, o, g, w, w, branch_scale=0.5)
+        return torch.autograd.grad((y, h), (x, o, g, w), (dy, dh))
+
+    same = lambda a, b: all(torch.equal(p, q) for p, q in zip(a, b))
+    want = step()
+    assert same(step(), want) and same(step(), want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(4):
+        with torch.no_grad():
+            for t in (x, o, g, w, dy, dh):
+                t.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(got, step())
