@@ -115,7 +115,9 @@ def fused_sgd(params, grads, momenta, lr, momentum=0.0, weight_decay=0.0,
 # the GPU, runs on the current stream, sums in float32 and rounds once; each
 # is differentiable once, with the same result in every run.  Calls may be
 # captured into a graph; a backward pass only while no eager graph of the same
-# leaves is alive, as with torch's own operators.
+# leaves is alive, as with torch's own operators.  A tracer (torch.jit.trace,
+# make_fx) cannot record them and is refused; torch.compile calls them as they
+# are.
 
 
 def embedding(weight: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,

@@ -8,10 +8,12 @@
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <array>
@@ -48,6 +50,21 @@ ElemType elem(at::ScalarType t) {
   return t == at::kFloat      ? ElemType::kF32
          : t == at::kBFloat16 ? ElemType::kBF16
                               : ElemType::kF16;
+}
+
+// A recorder would see the tensors that are made here and not the kernels that
+// fill them: its recording would give whatever their memory holds.
+void check_not_recorded(const char* op) {
+  using c10::impl::TorchDispatchModeKey;
+  bool recorded = torch::jit::tracer::isTracing() ||
+                  c10::impl::tls_is_dispatch_key_included(
+                      c10::DispatchKey::PreDispatch);
+  if (c10::impl::dispatch_mode_enabled())
+    for (const auto key : {TorchDispatchModeKey::FAKE,
+                           TorchDispatchModeKey::PROXY,
+                           TorchDispatchModeKey::FUNCTIONAL})
+      recorded |= c10::impl::TorchDispatchModeTLS::get_mode(key).has_value();
+  TORCH_CHECK(!recorded, op, ": cannot be recorded by a tracer");
 }
 
 void check_act(const Tensor& t, const char* op, const char* name) {
@@ -98,6 +115,7 @@ class OpNode : public torch::autograd::Node {
 
  protected:
   std::array<Tensor, N> kept(const char* op) {
+    check_not_recorded(op);
     TORCH_CHECK(!at::GradMode::is_enabled(), op,
                 ": its gradient cannot be differentiated again");
     const std::lock_guard<std::mutex> lock(mutex_);
@@ -216,6 +234,7 @@ Tensor embedding(const Tensor& weight, const Tensor& tokens, double scale,
                  std::optional<int64_t> padding_idx,
                  std::optional<at::ScalarType> out_dtype) {
   const char* op = "embedding";
+  check_not_recorded(op);
   check_act(weight, op, "weight");
   TORCH_CHECK(tokens.scalar_type() == at::kLong ||
                   tokens.scalar_type() == at::kInt,
@@ -522,6 +541,7 @@ Tensor contiguous(const OptTensor& t) {  // undefined where it is not given
 
 Tensor rms_norm(const Tensor& x, const OptTensor& weight, double eps) {
   const char* op = "rms_norm";
+  check_not_recorded(op);
   check_norm_input(x, op, "x");
   check_norm_weight(weight, x, op, "weight");
   TORCH_CHECK(eps >= 0, op, ": eps must not be negative");
@@ -539,6 +559,7 @@ std::tuple<Tensor, OptTensor> gated_residual_norm(
     const OptTensor& post_weight, const OptTensor& pre_weight,
     double residual_scale, double branch_scale, double eps) {
   const char* op = "gated_residual_norm";
+  check_not_recorded(op);
   check_norm_input(x, op, "x");
   check_act(branch, op, "branch");
   TORCH_CHECK(branch.scalar_type() == x.scalar_type(), op,
@@ -650,6 +671,7 @@ std::tuple<Tensor, Tensor> pack_rows(const Tensor& x) {
 }
 
 std::tuple<Tensor, Tensor> act8_pack_op(const Tensor& x) {
+  check_not_recorded("act8_pack");
   check_act8_input(x, "act8_pack", "x");
   check_device(x, x, "act8_pack", "x");
   at::NoGradGuard no_grad;
@@ -687,6 +709,7 @@ Tensor act8_unpack_op(const Tensor& codes, const Tensor& exps,
                       const std::vector<int64_t>& shape,
                       at::ScalarType dtype) {
   const char* op = "act8_unpack";
+  check_not_recorded(op);
   TORCH_CHECK(is_act_type(dtype), op,
               ": dtype must be float32, bfloat16 or float16, not ", dtype);
   TORCH_CHECK(!shape.empty(), op, ": the shape must have rows");
@@ -759,6 +782,7 @@ std::tuple<Tensor, OptTensor> act8_wgrad_op(const Tensor& dy,
                                             const std::vector<int64_t>& shape,
                                             at::ScalarType dtype, bool bias) {
   const char* op = "act8_wgrad";
+  check_not_recorded(op);
   check_act8_input(dy, op, "dy");
   TORCH_CHECK(dy.scalar_type() == dtype, op, ": dy must have the kept input's "
               "type ", dtype, ", not ", dy.scalar_type());
@@ -826,6 +850,7 @@ struct LinearAct8Node : OpNode<3> {
 Tensor linear_act8(const Tensor& x, const Tensor& weight,
                    const OptTensor& bias) {
   const char* op = "linear_act8";
+  check_not_recorded(op);
   check_act8_input(x, op, "x");
   check_act(weight, op, "weight");
   TORCH_CHECK(weight.scalar_type() == x.scalar_type(), op,
@@ -919,6 +944,7 @@ struct SiluAct8Node : OpNode<2> {
 
 Tensor silu_mul_act8(const Tensor& x) {
   const char* op = "silu_mul_act8";
+  check_not_recorded(op);
   check_act8_input(x, op, "x");
   TORCH_CHECK(x.size(-1) % 2 == 0, op,
               ": x must hold two halves in its last dimension, not ",

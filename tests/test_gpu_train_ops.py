@@ -357,3 +357,28 @@ def test_gradient_as_a_negated_view(which):
     got = torch.autograd.grad(y, leaves, torch._neg_view(dout),
                               allow_unused=True)
     assert all(a is b or torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_backward_in_a_recording_is_refused(which):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    f, leaves = _each_operator()[which]
+    y = f(*leaves)
+    used = leaves[0]
+    with pytest.raises(RuntimeError, match="cannot be recorded"):
+        make_fx(lambda d: torch.autograd.grad(y, used, d)[0])(
+            torch.ones_like(y))
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_inside_a_compiled_function(which):
+    """A compiled function calls the operators as they are."""
+    f, leaves = _each_operator()[which]
+    y = f(*leaves)
+    dout = torch.randn_like(y)
+    want = torch.autograd.grad(y, leaves, dout, allow_unused=True)
+    z = torch.compile(lambda *a: f(*a) * 2.0, backend="eager")(*leaves)
+    got = torch.autograd.grad(z, leaves, dout * 0.5, allow_unused=True)
+    assert torch.equal(z, y * 2.0)
+    assert all(a is b or torch.equal(a, b) for a, b in zip(got, want))

@@ -90,3 +90,39 @@ def _kept(rows=4, cols=40, pitch=64, groups=2, dtype=torch.bfloat16):
 def test_kept_refused(call, what):
     with pytest.raises(RuntimeError, match=what):
         call()
+
+
+RECORDED = [
+    lambda x: ops.embedding(x, TOK),
+    lambda x: ops.rms_norm(x),
+    lambda x: ops.gated_residual_norm(x, x)[0],
+    lambda x: ops.act8_pack(x).codes,
+    lambda x: ops.act8_unpack(_kept()) + x.sum(),
+    lambda x: ops.act8_wgrad(x, _kept(cols=8, pitch=32, groups=1))[0],
+    lambda x: ops.linear_act8(x, x),
+    lambda x: ops.silu_mul_act8(x),
+]
+
+
+@pytest.mark.parametrize("f", RECORDED)
+def test_recording_refused(f):
+    """A recording would hold the results' memory without what fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.ones(4, 8)
+    with pytest.raises(RuntimeError, match="cannot be recorded"):
+        torch.jit.trace(f, x)
+    for how in (dict(), dict(tracing_mode="fake"),
+                dict(tracing_mode="symbolic"), dict(pre_dispatch=True)):
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            make_fx(f, **how)(x)
+    with pytest.raises(RuntimeError, match="must"):
+        f(x)  # outside it, the call is refused for what is wrong with it
+
+
+def test_counting_modes_are_no_recording():
+    from torch.utils.flop_counter import FlopCounterMode
+
+    with FlopCounterMode(display=False):
+        with pytest.raises(RuntimeError, match="must be on the GPU"):
+            ops.rms_norm(torch.ones(4, 8))
