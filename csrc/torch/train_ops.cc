@@ -67,13 +67,25 @@ void check_not_recorded(const char* op) {
   TORCH_CHECK(!recorded, op, ": cannot be recorded by a tracer");
 }
 
-void check_act(const Tensor& t, const char* op, const char* name) {
-  TORCH_CHECK(t.defined(), op, ": ", name, " is missing");
+// Kernels read a tensor's memory: it has to be there, and to hold the values
+// themselves.  Wrappers of other tensors and tensors that only stand for zeros
+// have none.
+bool has_memory(const Tensor& t) {
+  return t.numel() == 0 || t.storage().data() != nullptr;
+}
+
+void check_plain(const Tensor& t, const char* op, const char* name) {
   TORCH_CHECK(t.layout() == at::kStrided, op, ": ", name, " must be dense");
-  TORCH_CHECK(is_act_type(t.scalar_type()), op, ": ", name,
-              " must be float32, bfloat16 or float16, not ", t.scalar_type());
   TORCH_CHECK(!t.is_neg(), op, ": ", name,
               " is a view that stands for its negative; resolve_neg() it");
+  TORCH_CHECK(has_memory(t), op, ": ", name, " holds no values of its own");
+}
+
+void check_act(const Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(t.defined(), op, ": ", name, " is missing");
+  TORCH_CHECK(is_act_type(t.scalar_type()), op, ": ", name,
+              " must be float32, bfloat16 or float16, not ", t.scalar_type());
+  check_plain(t, op, name);
 }
 
 void check_device(const Tensor& t, const Tensor& on, const char* op,
@@ -143,8 +155,15 @@ struct Rows {
   int64_t stride;
 };
 
+// A gradient as autograd gives it, in memory as it is.
+Tensor plain(const Tensor& given) {
+  if (given._is_zerotensor()) return at::zeros(given.sizes(), given.options());
+  TORCH_CHECK(has_memory(given), "a gradient holds no values of its own");
+  return given.resolve_neg();
+}
+
 Rows as_rows(const Tensor& given) {
-  const Tensor t = given.resolve_neg();
+  const Tensor t = plain(given);
   const int64_t dim = t.size(-1);
   bool ok = dim <= 1 || t.stride(-1) == 1;
   int64_t stride = dim, next = -1;
@@ -240,6 +259,7 @@ Tensor embedding(const Tensor& weight, const Tensor& tokens, double scale,
                   tokens.scalar_type() == at::kInt,
               op, ": tokens must be int64 or int32, not ",
               tokens.scalar_type());
+  check_plain(tokens, op, "tokens");
   const at::ScalarType out = out_dtype ? *out_dtype : weight.scalar_type();
   TORCH_CHECK(is_act_type(out), op,
               ": out_dtype must be float32, bfloat16 or float16, not ", out);
@@ -685,6 +705,8 @@ void check_codes(const Tensor& codes, const Tensor& exps, int64_t rows,
   TORCH_CHECK(codes.scalar_type() == at::kByte &&
                   exps.scalar_type() == at::kByte,
               op, ": codes and exponents must be bytes");
+  check_plain(codes, op, "codes");
+  check_plain(exps, op, "exponents");
   TORCH_CHECK(codes.dim() == 2 && codes.size(0) == rows &&
                   codes.size(1) == pitch && codes.is_contiguous(),
               op, ": codes must be contiguous [", rows, ", ", pitch, "], not ",
@@ -829,7 +851,7 @@ struct LinearAct8Node : OpNode<3> {
     const auto saved = kept("linear_act8");
     variable_list out(3);
     if (!grads[0].defined()) return out;
-    const Tensor& dy = grads[0];
+    const Tensor dy = plain(grads[0]);
     const c10::OptionalDeviceGuard guard(dy.device());
     if (task_should_compute_output(0)) {
       auto sizes = dy.sizes().vec();

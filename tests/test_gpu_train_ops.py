@@ -382,3 +382,12 @@ def test_inside_a_compiled_function(which):
     got = torch.autograd.grad(z, leaves, dout * 0.5, allow_unused=True)
     assert torch.equal(z, y * 2.0)
     assert all(a is b or torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_gradient_that_only_stands_for_zeros(which):
+    f, leaves = _each_operator()[which]
+    y = f(*leaves)
+    none = torch._efficientzerotensor(y.shape, device="cuda")
+    got = torch.autograd.grad(y, leaves, none, allow_unused=True)
+    assert all(v is None or (v == 0).all() for v in got)

@@ -126,3 +126,67 @@ def test_counting_modes_are_no_recording():
     with FlopCounterMode(display=False):
         with pytest.raises(RuntimeError, match="must be on the GPU"):
             ops.rms_norm(torch.ones(4, 8))
+
+
+class _Wrapper(torch.Tensor):
+    """A tensor around another one, with no memory of its own, as those of
+    torch.distributed.tensor are."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(
+            cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args, kwargs=None):
+        raise RuntimeError("the operator looked into a wrapper")
+
+
+def _zeros(*shape):
+    return torch._efficientzerotensor(shape)
+
+
+def _wrapped(*shape):
+    return _Wrapper(torch.zeros(*shape))
+
+
+def _byte(make, *shape):
+    if make is _zeros:
+        return torch._efficientzerotensor(shape, dtype=torch.uint8)
+    return _Wrapper(torch.zeros(*shape, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("make", [_zeros, _wrapped])
+@pytest.mark.parametrize("call,name", [
+    (lambda m, t: ops.embedding(m(4, 8), TOK), "weight"),
+    (lambda m, t: ops.rms_norm(m(4, 8)), "x"),
+    (lambda m, t: ops.rms_norm(t, m(8)), "weight"),
+    (lambda m, t: ops.gated_residual_norm(t, m(4, 8)), "branch"),
+    (lambda m, t: ops.gated_residual_norm(t, t, m(8)), "gate"),
+    (lambda m, t: ops.gated_residual_norm(t, t, None, m(8)), "post_weight"),
+    (lambda m, t: ops.gated_residual_norm(t, t, None, None, m(8)),
+     "pre_weight"),
+    (lambda m, t: ops.act8_pack(m(4, 8)), "x"),
+    (lambda m, t: ops.act8_wgrad(m(4, 8), _kept(dtype=torch.float32)), "dy"),
+    (lambda m, t: ops.act8_unpack(_kept()._replace(codes=_byte(m, 4, 64))),
+     "codes"),
+    (lambda m, t: ops.act8_unpack(_kept()._replace(exponents=_byte(m, 4, 2))),
+     "exponents"),
+    (lambda m, t: ops.linear_act8(m(4, 8), t), "x"),
+    (lambda m, t: ops.linear_act8(t, m(5, 8)), "weight"),
+    (lambda m, t: ops.linear_act8(t, t, m(4)), "bias"),
+    (lambda m, t: ops.silu_mul_act8(m(4, 8)), "x"),
+])
+def test_tensors_without_memory_refused(make, call, name):
+    with pytest.raises(RuntimeError, match=f"{name} holds no values"):
+        call(make, torch.zeros(4, 8))
+
+
+def test_tokens_without_memory_or_negated_refused():
+    for tok, what in (
+            (torch._efficientzerotensor((3,), dtype=torch.int64),
+             "tokens holds no values"),
+            (_Wrapper(TOK), "tokens holds no values"),
+            (torch._neg_view(TOK), "resolve_neg")):
+        with pytest.raises(RuntimeError, match=what):
+            ops.embedding(_bf(4, 8), tok)
