@@ -109,6 +109,13 @@ bool wants_grad(const char* op, std::initializer_list<const Tensor*> tensors) {
 
 const Tensor* get(const OptTensor& t) { return t ? &*t : nullptr; }
 
+// A tensor that autograd gives, with its values in memory as they are.
+Tensor plain(const Tensor& given) {
+  if (given._is_zerotensor()) return at::zeros(given.sizes(), given.options());
+  TORCH_CHECK(has_memory(given), "a gradient or a kept tensor holds no values of its own");
+  return given.resolve_neg();
+}
+
 // An operator's backward pass: a node of the graph that keeps N tensors.  As a
 // node of its own it has its numbers as members; through torch's Function, with
 // its context of named values, a call with a gradient took 5 us longer.
@@ -118,6 +125,8 @@ class OpNode : public torch::autograd::Node {
   // Only once t has been written: a hook may copy it here.
   void keep(size_t i, const Tensor& t) {
     saved_[i] = torch::autograd::SavedVariable(t, false);
+    if (saved_[i].has_hooks())
+      saved_as_[i] = {t.options(), t.sizes().vec(), t.is_contiguous()};
   }
 
   void release_variables() override {
@@ -132,12 +141,39 @@ class OpNode : public torch::autograd::Node {
                 ": its gradient cannot be differentiated again");
     const std::lock_guard<std::mutex> lock(mutex_);
     std::array<Tensor, N> t;
-    for (size_t i = 0; i < N; i++) t[i] = saved_[i].unpack();
+    for (size_t i = 0; i < N; i++) {
+      t[i] = saved_[i].unpack();
+      if (saved_[i].has_hooks()) t[i] = as_saved(op, t[i], saved_as_[i]);
+    }
     return t;
   }
 
  private:
+  struct Meta {
+    at::TensorOptions options;
+    std::vector<int64_t> sizes;
+    bool contiguous;
+  };
+
+  // What a hook gave back for a kept tensor: the kernels read it by the type,
+  // place and sizes that it had, and take rows and codes as aligned as torch's
+  // allocator makes them.
+  static Tensor as_saved(const char* op, const Tensor& t, const Meta& m) {
+    TORCH_CHECK(t.layout() == at::kStrided &&
+                    t.scalar_type() == m.options.dtype().toScalarType() &&
+                    t.device() == m.options.device() && t.sizes() == m.sizes,
+                op, ": a hook on kept tensors gave back ", t.scalar_type(), " ",
+                t.sizes(), " on ", t.device(), " for ",
+                m.options.dtype().toScalarType(), " ",
+                at::IntArrayRef(m.sizes), " on ", m.options.device());
+    Tensor own = plain(t);
+    if (m.contiguous) own = own.contiguous();
+    const bool aligned = ((uintptr_t)own.const_data_ptr() & 15) == 0;
+    return aligned || !m.contiguous ? own : own.clone();
+  }
+
   std::array<torch::autograd::SavedVariable, N> saved_;
+  std::array<Meta, N> saved_as_;
 };
 
 // A node that gives gradients to `inputs`, in their order.
@@ -154,13 +190,6 @@ struct Rows {
   Tensor t;
   int64_t stride;
 };
-
-// A gradient as autograd gives it, in memory as it is.
-Tensor plain(const Tensor& given) {
-  if (given._is_zerotensor()) return at::zeros(given.sizes(), given.options());
-  TORCH_CHECK(has_memory(given), "a gradient holds no values of its own");
-  return given.resolve_neg();
-}
 
 Rows as_rows(const Tensor& given) {
   const Tensor t = plain(given);

@@ -391,3 +391,58 @@ def test_gradient_that_only_stands_for_zeros(which):
     none = torch._efficientzerotensor(y.shape, device="cuda")
     got = torch.autograd.grad(y, leaves, none, allow_unused=True)
     assert all(v is None or (v == 0).all() for v in got)
+
+
+def _through(f, leaves, unpack):
+    """f of the leaves, with a hook that gives back unpack(kept tensor)."""
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(),
+                                                  unpack):
+        return f(*leaves)
+
+
+@pytest.mark.parametrize("which", range(6))
+@pytest.mark.parametrize("unpack", [
+    lambda t: t.to(BF if t.dtype == torch.float32 else torch.int16),
+    lambda t: t.cpu(),
+    lambda t: t.reshape(-1)[:1],
+    lambda t: t[None],
+    lambda t: t.to_sparse(),
+])
+def test_hook_that_gives_back_another_tensor(which, unpack):
+    """Another type, place or size than what was kept is refused: the kernels
+    would read past its end."""
+    f, leaves = _each_operator()[which]
+    y = _through(f, leaves, unpack)
+    with pytest.raises(RuntimeError, match="hook on kept tensors"):
+        torch.autograd.grad(y.sum(), leaves, allow_unused=True)
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_hook_that_gives_back_another_layout(which):
+    """The same values in other strides, or away from 16 bytes."""
+    f, leaves = _each_operator()[which]
+    y = f(*leaves)
+    dout = torch.randn_like(y)
+    want = torch.autograd.grad(y, leaves, dout, allow_unused=True)
+
+    def apart(t):
+        return torch.stack([t, t], -1)[..., 0]
+
+    def shifted(t):
+        flat = t.reshape(-1)
+        return torch.cat([flat[:1], flat])[1:].view(t.shape)
+
+    def turned(t):
+        return t.t().contiguous().t() if t.dim() == 2 else t
+
+    def stands_for_zeros(t):
+        return torch._efficientzerotensor(t.shape, dtype=t.dtype,
+                                          device=t.device)
+
+    for unpack in (apart, shifted, turned):
+        got = torch.autograd.grad(_through(f, leaves, unpack), leaves, dout,
+                                  allow_unused=True)
+        assert all(a is b or torch.equal(a, b) for a, b in zip(got, want))
+    torch.autograd.grad(_through(f, leaves, stands_for_zeros), leaves, dout,
+                        allow_unused=True)
+    torch.cuda.synchronize()
