@@ -7,8 +7,12 @@ extension raises — the HIP path must never silently fall back to eager.
 
 from __future__ import annotations
 
+import contextlib
+import fcntl
+import hashlib
 import importlib.util
 import os
+import sys
 from pathlib import Path
 from typing import NamedTuple
 
@@ -18,6 +22,12 @@ from .. import REPO_ROOT
 
 _C = None
 _ERR: Exception | None = None
+
+_CXX_FLAGS = ["-O3"]
+# packed fp32 instructions stay out of every kernel: some of their forms have
+# given wrong results on this hardware
+_HIP_FLAGS = ["-O3", "-Xclang", "-target-feature", "-Xclang",
+              "-packed-fp32-ops"]
 
 
 def _sources() -> list[Path]:
@@ -41,22 +51,68 @@ def _import_built(lib: Path):
     return module
 
 
+def _wanted(sources: list[Path]) -> str:
+    """What the built extension depends on, as a hash: its sources, compiler
+    flags and architecture, and the torch and Python that load it."""
+    h = hashlib.sha256()
+    for part in (_CXX_FLAGS, _HIP_FLAGS, os.environ["PYTORCH_ROCM_ARCH"],
+                 torch.__version__, torch.version.git_version,
+                 torch.version.hip, sys.version_info[:2]):
+        h.update(repr(part).encode() + b"\0")
+    headers = sorted((REPO_ROOT / "csrc" / "hip").glob("*.h"))
+    for p in sources + headers:
+        h.update(p.name.encode() + b"\0" + p.read_bytes() + b"\0")
+    return h.hexdigest()
+
+
+@contextlib.contextmanager
+def _locked(build_dir: Path, how: int):
+    """The build directory's lock: shared to load, exclusive to build.  It ends
+    with its process, and a directory that cannot be written to needs none."""
+    try:
+        build_dir.mkdir(parents=True, exist_ok=True)
+        file = open(build_dir / "baguanet_C.lock", "a")
+    except OSError:
+        yield
+        return
+    with file:
+        fcntl.flock(file, how)
+        yield
+
+
 def build_extension(verbose: bool = False, force: bool = False):
-    """Load the extension from its in-tree build dir, compiled first if it is
-    missing or older than its sources, or always with ``force``."""
+    """Load the extension from its in-tree build dir, compiled first if there
+    is none built from these sources with these flags, or always with
+    ``force``."""
     global _C, _ERR
     if _C is not None and not force:
         return _C
+    os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
     build_dir = REPO_ROOT / "build" / "torch_ext"
     lib = build_dir / "baguanet_C.so"
+    # written after a build: a library without it may be half written
+    stamp = build_dir / "baguanet_C.stamp"
     try:
         sources = _sources()
-        headers = list((REPO_ROOT / "csrc" / "hip").glob("*.h"))
-        newest = max(p.stat().st_mtime for p in sources + headers)
-        if force or not lib.exists() or lib.stat().st_mtime < newest:
-            _C = _compile(build_dir, sources, verbose, force)
-        else:
-            _C = _import_built(lib)
+        wanted = _wanted(sources)
+
+        def built() -> bool:
+            return (lib.exists() and stamp.exists()
+                    and stamp.read_text() == wanted)
+
+        if not force:
+            with _locked(build_dir, fcntl.LOCK_SH):
+                if built():
+                    _C = _import_built(lib)
+                    return _C
+        with _locked(build_dir, fcntl.LOCK_EX):
+            if not force and built():  # by another process, meanwhile
+                _C = _import_built(lib)
+                return _C
+            stamp.unlink(missing_ok=True)
+            module = _compile(build_dir, sources, verbose, force)
+            stamp.write_text(wanted)
+            _C = module
     except Exception as e:  # pragma: no cover
         _ERR = e
         raise
@@ -67,8 +123,6 @@ def _compile(build_dir: Path, sources: list[Path], verbose: bool,
              force: bool):
     from torch.utils import cpp_extension
 
-    os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
-    build_dir.mkdir(parents=True, exist_ok=True)
     if force:
         for built in build_dir.glob("*.o"):
             built.unlink()
@@ -76,11 +130,8 @@ def _compile(build_dir: Path, sources: list[Path], verbose: bool,
         name="baguanet_C",
         sources=[str(p) for p in sources],
         build_directory=str(build_dir),
-        extra_cflags=["-O3"],
-        # packed fp32 instructions stay out of every kernel: some of their
-        # forms have given wrong results on this hardware
-        extra_cuda_cflags=["-O3", "-Xclang", "-target-feature", "-Xclang",
-                           "-packed-fp32-ops"],
+        extra_cflags=_CXX_FLAGS,
+        extra_cuda_cflags=_HIP_FLAGS,
         verbose=verbose,
     )
 
