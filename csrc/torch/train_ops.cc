@@ -16,6 +16,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <array>
 #include <memory>
 #include <mutex>
@@ -764,8 +765,15 @@ Tensor act8_unpack_op(const Tensor& codes, const Tensor& exps,
   TORCH_CHECK(is_act_type(dtype), op,
               ": dtype must be float32, bfloat16 or float16, not ", dtype);
   TORCH_CHECK(!shape.empty(), op, ": the shape must have rows");
-  int64_t rows = 1;
-  for (size_t d = 0; d + 1 < shape.size(); d++) rows *= shape[d];
+  for (const int64_t n : shape)
+    TORCH_CHECK(n >= 0, op, ": a shape of ", at::IntArrayRef(shape));
+  const auto lead = at::IntArrayRef(shape).slice(0, shape.size() - 1);
+  int64_t rows = std::find(lead.begin(), lead.end(), 0) == lead.end();
+  for (const int64_t n : lead) {
+    TORCH_CHECK(rows == 0 || n <= kMaxRows / rows, op, ": at most 2^30 rows");
+    rows *= n;
+  }
+  TORCH_CHECK(shape.back() <= kMaxRows, op, ": at most 2^30 columns");
   check_codes(codes, exps, rows, shape.back(), op);
   check_device(codes, codes, op, "codes");
   check_device(exps, codes, op, "exponents");

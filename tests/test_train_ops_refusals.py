@@ -190,3 +190,26 @@ def test_tokens_without_memory_or_negated_refused():
             (torch._neg_view(TOK), "resolve_neg")):
         with pytest.raises(RuntimeError, match=what):
             ops.embedding(_bf(4, 8), tok)
+
+
+@pytest.mark.parametrize("shape", [(2 ** 31, 0), (2 ** 16, 2 ** 15, 0),
+                                   (2 ** 33, 2 ** 31, 0)])
+def test_unpack_of_too_many_rows_refused(shape):
+    """As act8_pack: the kernels count rows in 32 bits."""
+    rows = 1
+    for n in shape[:-1]:
+        rows = rows * n % 2 ** 64
+    none = torch.empty(rows, 0, dtype=torch.uint8)
+    kept = ops.Act8(none, none, torch.Size(shape), torch.float32)
+    with pytest.raises(RuntimeError, match=r"at most 2\^30 rows"):
+        ops.act8_unpack(kept)
+
+
+def test_unpack_of_no_shape_refused():
+    for shape in ((4, -40), (-4, 40), (0, -1)):
+        with pytest.raises(RuntimeError, match="a shape of"):
+            ops.act8_unpack(_kept()._replace(shape=shape))
+    with pytest.raises(RuntimeError, match="codes must be on the GPU"):
+        none = torch.empty(0, 64, dtype=torch.uint8)
+        ops.act8_unpack(ops.Act8(none, none[:, :2], (2 ** 29, 0, 8, 40),
+                                 torch.float32))
