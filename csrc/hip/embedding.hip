@@ -608,8 +608,10 @@ hipError_t embedding_backward(const EmbeddingBwd& a, hipStream_t stream) {
   const int64_t teams = kBlock / ch.tpr;
   const int64_t blocks = (ch.count * ch.tiles + teams - 1) / teams;
   // the largest launches: the sums', and one that zeroes a part of dW
-  const int64_t zeros = a.vocab * a.dim / (kSortBlock * kZeroPieces * 4);
-  if (blocks > kMaxBlocks || zeros > kMaxBlocks / 2)
+  static_assert(kEmbeddingMaxGrad / (kSortBlock * kZeroPieces * 4) <=
+                    kMaxBlocks / 2 + 1,
+                "launches that zero a part of dW");
+  if (blocks > kMaxBlocks || a.vocab > kEmbeddingMaxGrad / a.dim)
     return hipErrorInvalidValue;
   char* ws = (char*)a.workspace;
   Sorted buf[2];

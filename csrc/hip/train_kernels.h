@@ -35,6 +35,9 @@ struct EmbeddingBwd {
   bool tok64;
   ElemType dtype, wtype;
 };
+// Elements that a table with a gradient may have, fewer than: the launches that
+// clear it are counted in 32 bits.
+constexpr int64_t kEmbeddingMaxGrad = int64_t(1) << 35;
 size_t embedding_workspace(int64_t vocab, int64_t dim, int64_t n);
 hipError_t embedding_backward(const EmbeddingBwd& a, hipStream_t stream);
 

@@ -113,7 +113,8 @@ const Tensor* get(const OptTensor& t) { return t ? &*t : nullptr; }
 // A tensor that autograd gives, with its values in memory as they are.
 Tensor plain(const Tensor& given) {
   if (given._is_zerotensor()) return at::zeros(given.sizes(), given.options());
-  TORCH_CHECK(has_memory(given), "a gradient or a kept tensor holds no values of its own");
+  TORCH_CHECK(has_memory(given),
+              "a gradient or a kept tensor holds no values of its own");
   return given.resolve_neg();
 }
 
@@ -298,6 +299,10 @@ Tensor embedding(const Tensor& weight, const Tensor& tokens, double scale,
   const int64_t vocab = weight.size(0);
   TORCH_CHECK(vocab <= kMaxRows && tokens.numel() <= kMaxRows, op,
               ": at most 2^30 rows and tokens");
+  const bool grad = at::GradMode::is_enabled() && weight.requires_grad();
+  TORCH_CHECK(!grad || vocab == 0 ||
+                  weight.size(1) < kEmbeddingMaxGrad / vocab,
+              op, ": a table with a gradient has fewer than 2^35 elements");
   int64_t padding = -1;
   if (padding_idx) {
     padding = *padding_idx < 0 ? *padding_idx + vocab : *padding_idx;

@@ -213,3 +213,18 @@ def test_unpack_of_no_shape_refused():
         none = torch.empty(0, 64, dtype=torch.uint8)
         ops.act8_unpack(ops.Act8(none, none[:, :2], (2 ** 29, 0, 8, 40),
                                  torch.float32))
+
+
+@pytest.mark.parametrize("rows,cols", [(2 ** 20, 2 ** 15), (2 ** 30, 2 ** 32),
+                                       (7, 2 ** 33)])
+def test_table_too_large_for_its_gradient_refused(rows, cols):
+    """Before the lookup, not in the backward pass that cannot do it."""
+    one = torch.zeros(1, 1)
+    table = one.expand(rows, cols).requires_grad_()
+    with pytest.raises(RuntimeError, match=r"fewer than 2\^35"):
+        ops.embedding(table, TOK)
+    for call in (lambda: ops.embedding(table.detach(), TOK),
+                 lambda: ops.embedding(one.expand(2 ** 20, 2 ** 15 - 1)
+                                       .requires_grad_(), TOK)):
+        with pytest.raises(RuntimeError, match="must be on the GPU"):
+            call()
