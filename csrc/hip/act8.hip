@@ -91,9 +91,19 @@ __global__ __launch_bounds__(kBlock) void act8_unpack_kernel(Act8Move a,
 // values a', b' and s = 1 / (1 + exp(-a')):
 //   da = dout * b' * s * (1 + a' * (1 - s))     db = dout * a' * s
 
-__device__ inline float sigmoid(float a) {
-  return __builtin_amdgcn_rcpf(1.f + expf(-a));
-}
+// s and 1 - s.  With h = exp(-|a| / 2), s is 1 / (1 + h^2) or h^2 times that,
+// and stays in two factors: far below 0 it is less than fp32's smallest normal
+// number where its product with a and b is not.
+struct Sigmoid {
+  float s0, s1, rest;
+  __device__ inline explicit Sigmoid(float a) {
+    const float h = expf(-0.5f * fabsf(a)), e = h * h;
+    const float r = __builtin_amdgcn_rcpf(1.f + e);
+    s0 = a < 0.f ? h : r;
+    s1 = a < 0.f ? h * r : 1.f;
+    rest = a < 0.f ? r : e * r;
+  }
+};
 
 template <typename T>
 __global__ __launch_bounds__(kBlock) void silu_forward_kernel(SiluAct8 p,
@@ -113,7 +123,10 @@ __global__ __launch_bounds__(kBlock) void silu_forward_kernel(SiluAct8 p,
         a = load_upto(src + c, m);
         b = load_upto(src + p.cols + c, m);
 #pragma unroll
-        for (int i = 0; i < kVec; i++) o[i] = a[i] * sigmoid(a[i]) * b[i];
+        for (int i = 0; i < kVec; i++) {
+          const Sigmoid s(a[i]);
+          o[i] = a[i] * s.s0 * b[i] * s.s1;
+        }
         store_upto((T*)p.out + r * p.cols + c, o, m);
       }
       if (!p.codes) continue;
@@ -152,9 +165,9 @@ __global__ __launch_bounds__(kBlock) void silu_backward_kernel(SiluAct8 p,
       float8 da, db;
 #pragma unroll
       for (int i = 0; i < kVec; i++) {
-        const float s = sigmoid(a[i]);
-        da[i] = d[i] * b[i] * s * (1.f + a[i] * (1.f - s));
-        db[i] = d[i] * a[i] * s;
+        const Sigmoid s(a[i]);
+        da[i] = d[i] * b[i] * s.s0 * (1.f + a[i] * s.rest) * s.s1;
+        db[i] = d[i] * s.s0 * a[i] * s.s1;
       }
       T* dst = (T*)p.dx + r * 2 * p.cols + c;
       store_upto(dst, da, m);

@@ -446,3 +446,33 @@ def test_same_every_time_streams_and_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert equal(got, step())
+
+
+@pytest.mark.parametrize("big", [1.0, 3e20, 2e37])
+def test_silu_of_tails(big):
+    """Where 1 / (1 + exp(-a)) itself is below fp32's smallest normal number
+    and the product with b is not: the factors are multiplied apart.  exp is
+    within a step of 2**-23 and enters twice, and six more operations follow."""
+    from baguanet import ops
+
+    a = -torch.arange(60, 124).float() * 0.875 - torch.rand(
+        5, 64, generator=torch.Generator().manual_seed(1))
+    b = (1 + torch.rand(5, 64, generator=torch.Generator().manual_seed(2)))
+    x = torch.cat([a, b * big], -1)
+    g = rows((5, 64), F32, 3, wild=False)
+    xd = x.cuda().requires_grad_()
+    out = ops.silu_mul_act8(xd)
+    (dx,) = torch.autograd.grad(out, xd, g.cuda())
+    a, b = x.double().chunk(2, -1)
+    # half a step among the numbers below the smallest normal one is 2**-150
+    def near(got, ref, rel):
+        off = (got.detach().double().cpu() - ref).abs()
+        assert (off <= ref.abs() * rel + 8 * 2.0 ** -150).all(), (
+            off / ref.abs()).max()
+
+    near(out, a / (1 + (-a).exp()) * b, 16 * U)
+    a, b = (kept(v) for v in x.chunk(2, -1))
+    s, d = 1 / (1 + (-a).exp()), g.double()
+    da, db = dx.chunk(2, -1)
+    near(da, d * b * s * (1 + a * (1 - s)), 24 * U)
+    near(db, d * a * s, 16 * U)
