@@ -196,7 +196,7 @@ void act8_wgrad_kernel(Product p) {
   constexpr int kPassK = kTM * kTK / 8 / kThreads;
   constexpr int kRowsN = kTM / kPassN, kRowsK = kTM / kPassK;  // of a pass
   constexpr int kTile = kTM * (kTN + kTK);  // both operands' tiles
-  __shared__ __attribute__((aligned(16))) short lds[2 * kTile];
+  __shared__ __attribute__((aligned(alignof(float8)))) short lds[2 * kTile];
   int tn, tk;
   pick_tile(p.part, tn, tk);
   const int64_t n0 = p.part.n0 + (int64_t)tn * kTN;

@@ -421,7 +421,7 @@ __global__ __launch_bounds__(kJoinBlock) void embedding_join_kernel(
   constexpr int kWaves = kJoinBlock / kWave, kRuns = kMany ? kWaves : 1;
   constexpr int kLanes = kMany ? kWave : 128;
   __shared__ int wave_end[kWaves], many[kRuns];
-  __shared__ float joint[kJoinBlock * kVec];
+  __shared__ float8 joint[kJoinBlock];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int tpr = ch.tpr < kLanes ? ch.tpr : kLanes;
   const int team = threadIdx.x / tpr, in = threadIdx.x % tpr;
@@ -505,12 +505,12 @@ __global__ __launch_bounds__(kJoinBlock) void embedding_join_kernel(
         __syncthreads();
       }
       float8 acc = add_parts(chunk, parts, at, team, teams);
-      *(float8*)&joint[threadIdx.x * kVec] = acc;
+      joint[threadIdx.x] = acc;
       __syncthreads();
       if (team == 0) {
         const int used = parts < teams ? (int)parts : teams;
         for (int t = 1; t < used; t++)
-          acc += *(const float8*)&joint[(t * tpr + in) * kVec];
+          acc += joint[t * tpr + in];
         c.store((W*)a.dweight + (int64_t)key * a.dim + at, acc * a.scale);
       }
       __syncthreads();
