@@ -236,9 +236,10 @@ def act8_pack(x: torch.Tensor) -> Act8:
 
     Groups of 32 neighbours of a row share a power of two that brings the
     largest to at most 448; each value is then an e4m3 number.  A value is
-    off by at most 1/16 of itself, or by 2**-19 of its group's largest if
-    that is more.  NaN and infinities are kept as NaN.  The copy takes 33
-    bytes for 32 values and no part in autograd.
+    off by at most 1/16 of itself, or, if that is more, by 2**-10 / 224
+    (2**-17.8) of its group's largest; float32 and bfloat16 values are off by
+    up to 2**-127 whatever their group holds.  NaN and infinities are kept as
+    NaN.  The copy takes 33 bytes for 32 values and no part in autograd.
     """
     codes, exponents = _load().act8_pack(x)
     return Act8(codes, exponents, x.shape, x.dtype)

@@ -476,3 +476,36 @@ def test_silu_of_tails(big):
     da, db = dx.chunk(2, -1)
     near(da, d * b * s * (1 + a * (1 - s)), 24 * U)
     near(db, d * a * s, 16 * U)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_documented_error_of_kept_values(dtype):
+    """At most 1/16 of the value, 2**-10 / 224 of its group's largest or, but
+    for fp16, 2**-127, whichever is most.  In a group whose largest is just
+    above 224 a step's half is 2**-10, and values just below it become 0."""
+    from baguanet import ops
+
+    top = torch.tensor([224.5, 225.0, 240.0, 256.0, 256.5, 300.0, 447.0, 448.0,
+                        448.5, 449.0]).to(dtype).double()
+    below = torch.cat([torch.tensor([0.99, 1.01, 1.49, 1.51, 2.49, 2.51, 3.0])
+                       * 2.0 ** e for e in range(-12, 0)])
+    g = torch.Generator().manual_seed(2)
+    wide = torch.exp2(torch.rand(len(top), 60, generator=g) * 24 - 16)
+    x = torch.cat([below.expand(len(top), -1), wide], 1).double()
+    n = x.shape[1] // 31
+    x = torch.cat([top[:, None, None].expand(-1, n, 1),
+                   x[:, :n * 31].reshape(len(top), n, 31)], -1).flatten(1)
+    powers = (0, -6) if dtype == HF else (0, 100, -100, -125, -135)
+    for p in powers:
+        v = (x * 2.0 ** p).to(dtype)
+        got = ops.act8_unpack(ops.act8_pack(v.cuda())).double().cpu()
+        v = v.double()
+        most = v.reshape(len(v), -1, 32).amax(-1, keepdim=True)
+        most = most.expand(-1, -1, 32).reshape(v.shape)
+        bound = torch.maximum(v / 16, most * 2.0 ** -10 / 224)
+        if dtype != HF:
+            bound = bound.clamp_min(2.0 ** -127)
+        assert ((got - v).abs() <= bound).all()
+        if p == 0:  # values come near the second bound
+            worst = ((got - v).abs() / most)[v < most / 2 ** 16].max()
+            assert worst > 0.9 * 2.0 ** -10 / 224
