@@ -509,3 +509,91 @@ def test_documented_error_of_kept_values(dtype):
         if p == 0:  # values come near the second bound
             worst = ((got - v).abs() / most)[v < most / 2 ** 16].max()
             assert worst > 0.9 * 2.0 ** -10 / 224
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("bias", [True, False])
+def test_wgrad_of_gradients_below_the_smallest_normal(dtype, bias):
+    """Gradients without loss scaling: among fp16's numbers below 2**-14 (or
+    bf16's below 2**-126) a product is as exact as any other."""
+    from baguanet import ops
+
+    m, n, k = 300, 140, 96
+    g = torch.Generator().manual_seed(6)
+    low = torch.finfo(dtype).smallest_normal
+    step = low * torch.finfo(dtype).eps
+    whole = torch.randint(-20, 21, (m, n), generator=g)
+    dy = (whole.double() * step).to(dtype)
+    assert (dy != 0).any() and (dy.abs().double() < low).all()
+    # whole numbers of at most 3 bits times 2**8 and 2**13: the products' sums
+    # are exact in fp32 and come out above the smallest normal number
+    x = torch.randint(-7, 8, (m, k), generator=g).float() * 2.0 ** 8
+    x[:, ::3] *= 2.0 ** 5
+    x = x.to(dtype)
+    kept_x = ops.act8_pack(x.cuda())
+    assert torch.equal(ops.act8_unpack(kept_x).cpu(), x)
+    dw, db = ops.act8_wgrad(dy.cuda(), kept_x, bias=bias)
+    d = dy.double()
+    within_exact = lambda got, ref: torch.equal(got.cpu(), ref.to(dtype))
+    assert within_exact(dw, d.t() @ x.double())
+    assert not bias or within_exact(db, d.sum(0))
+    dw, _ = ops.act8_wgrad(dy.float().cuda(), ops.act8_pack(x.float().cuda()))
+    want = d.t() @ x.double()
+    if dtype == HF:  # ordinary numbers of fp32
+        assert torch.equal(dw.double().cpu(), want)
+
+
+def test_wgrad_of_fp32_down_to_its_smallest():
+    """Three bf16 numbers of 8 bits hold an fp32 number from 2**-110 on; below
+    it what their smallest, 2**-133, cannot hold is lost: less than that for
+    each value."""
+    from baguanet import ops
+
+    g = torch.Generator().manual_seed(8)
+    e = torch.arange(-149, 128).double()
+    dy = (torch.rand(len(e), generator=g).double() + 1) * torch.exp2(e)
+    dy = torch.cat([dy.float(), -dy.float()])[:, None]
+    n = len(dy)
+    x = torch.eye(n)
+    dw, _ = ops.act8_wgrad(dy.cuda(), ops.act8_pack(x.cuda()))
+    want = dy.double().t()
+    assert ((dw.double().cpu() - want).abs()
+            <= want.abs() * 4 * U + 2.0 ** -133).all()
+
+
+def test_linear_act8_does_not_hold_its_input():
+    """What a graph keeps of a layer's input that is not kept elsewhere: the
+    codes, no less and no more."""
+    from baguanet import ops
+
+    w = torch.randn(64, 4096, device="cuda", dtype=BF, requires_grad=True)
+    ops.linear_act8(torch.randn(8, 4096, device="cuda", dtype=BF), w)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    x = torch.randn(8192, 4096, device="cuda", dtype=BF)
+    y = ops.linear_act8(x, w)
+    values = x.numel()
+    del x
+    held = torch.cuda.memory_allocated() - before - y.nbytes
+    # torch rounds each of the two blocks up to 512 bytes
+    assert values * 33 / 32 <= held <= values * 33 / 32 + 2 * 512
+    (dw,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    del y
+    assert torch.cuda.memory_allocated() - before - dw.nbytes <= 512
+
+
+def test_silu_holds_codes_only():
+    from baguanet import ops
+
+    ops.silu_mul_act8(torch.randn(8, 64, device="cuda", dtype=BF,
+                                  requires_grad=True))
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    leaf = torch.randn(4096, 4096, device="cuda", dtype=BF, requires_grad=True)
+    x = leaf * 1.0
+    y = ops.silu_mul_act8(x)
+    values, own = x.numel(), leaf.nbytes + y.nbytes
+    del x
+    held = torch.cuda.memory_allocated() - before - own
+    # multiplied by a plain number: torch keeps nothing for that
+    assert values * 33 / 32 <= held <= values * 33 / 32 + 4 * 512

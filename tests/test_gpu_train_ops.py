@@ -446,3 +446,23 @@ def test_hook_that_gives_back_another_layout(which):
     torch.autograd.grad(_through(f, leaves, stands_for_zeros), leaves, dout,
                         allow_unused=True)
     torch.cuda.synchronize()
+
+
+def test_block_holds_its_codes_outputs_and_branch():
+    """A whole block's graph to a few of the allocator's 512 bytes: neither
+    the linear layers' inputs nor the activation's result are in it."""
+    torch.manual_seed(0)
+    rows, dim, hidden = 4096, 1024, 2048
+    block = Block(dim, hidden, BF).cuda()
+    x = torch.randn(rows, dim, device="cuda").to(BF).requires_grad_()
+    h = torch.randn(rows, dim, device="cuda").to(BF).requires_grad_()
+    block(x[:8].detach(), h[:8].detach())
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    out = block(x, h)
+    now = torch.cuda.memory_allocated() - before
+    # y, h and the branch in 2 bytes; two numbers a row of the norms; 33/32 of
+    # a byte for the inputs of both layers and both halves of the activation's
+    kept = rows * (6 * dim + 8 + 33 / 32 * (dim + hidden + 2 * hidden))
+    assert kept <= now <= kept + 16 * 512
+    del out
