@@ -421,7 +421,8 @@ __global__ __launch_bounds__(kJoinBlock) void embedding_join_kernel(
   constexpr int kWaves = kJoinBlock / kWave, kRuns = kMany ? kWaves : 1;
   constexpr int kLanes = kMany ? kWave : 128;
   __shared__ int wave_end[kWaves], many[kRuns];
-  __shared__ float8 joint[kJoinBlock];
+  __shared__ __attribute__((aligned(alignof(float8)))) float
+      joint[kJoinBlock * kVec];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int tpr = ch.tpr < kLanes ? ch.tpr : kLanes;
   const int team = threadIdx.x / tpr, in = threadIdx.x % tpr;
@@ -505,12 +506,12 @@ __global__ __launch_bounds__(kJoinBlock) void embedding_join_kernel(
         __syncthreads();
       }
       float8 acc = add_parts(chunk, parts, at, team, teams);
-      joint[threadIdx.x] = acc;
+      *(float8*)&joint[threadIdx.x * kVec] = acc;
       __syncthreads();
       if (team == 0) {
         const int used = parts < teams ? (int)parts : teams;
         for (int t = 1; t < used; t++)
-          acc += joint[t * tpr + in];
+          acc += *(const float8*)&joint[(t * tpr + in) * kVec];
         c.store((W*)a.dweight + (int64_t)key * a.dim + at, acc * a.scale);
       }
       __syncthreads();

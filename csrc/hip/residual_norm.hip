@@ -175,11 +175,12 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
   constexpr int kTeams = block_of<TPR>() / TPR;
   __shared__ float red[2][3 * (TPR / kWave)];
   // the teams' column sums on their way to the first team
-  __shared__ float8 joint[kTeams > 1 ? kTeams - 1 : 1]
-                         [kTeams > 1 ? TPR * VPT : 1];
+  __shared__ __attribute__((aligned(alignof(float8)))) float
+      joint[kTeams > 1 ? kTeams - 1 : 1][kTeams > 1 ? TPR * VPT * kVec : 1];
   // wide rows: sums over rows that registers have no room for, for each lane
   constexpr bool kWide = TPR * VPT > 1024;
-  __shared__ float8 held[kWide ? 2 * TPR * VPT : 1];
+  __shared__ __attribute__((aligned(alignof(float8)))) float
+      held[kWide ? 2 * TPR * VPT * kVec : 1];
   constexpr bool kSeam = kind != Seam::kAny;
   const bool has_branch = kSeam || a.branch, has_post = kSeam || a.post;
   const bool has_dy = kSeam || a.dy, has_dh = kSeam || a.dh;
@@ -197,7 +198,7 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
   // wide rows read them again at each use
   float8 pre[VPT], coef[VPT], acc_pre[VPT], acc_post[VPT];
   auto held_at = [&](int what, int j) -> float8& {
-    return held[(what * VPT + j) * TPR + lane];
+    return *(float8*)&held[((what * VPT + j) * TPR + lane) * kVec];
   };
   auto add_pre = [&](int j, float8 v) {
     if constexpr (kWide)
@@ -237,14 +238,14 @@ __global__ __launch_bounds__(block_of<TPR>()) void norm_backward_kernel(
       if (team > 0) {
 #pragma unroll
         for (int j = 0; j < VPT; j++)
-          joint[team - 1][j * TPR + lane] = v[j];
+          *(float8*)&joint[team - 1][(j * TPR + lane) * kVec] = v[j];
       }
       __syncthreads();
       if (team == 0) {
         for (int t = 0; t < kTeams - 1; t++) {
 #pragma unroll
           for (int j = 0; j < VPT; j++)
-            v[j] += joint[t][j * TPR + lane];
+            v[j] += *(const float8*)&joint[t][(j * TPR + lane) * kVec];
         }
       }
     }
