@@ -23,6 +23,7 @@ from .. import REPO_ROOT
 _C = None
 _ERR: Exception | None = None
 
+_ARCH = "PYTORCH_ROCM_ARCH"
 _CXX_FLAGS = ["-O3"]
 # packed fp32 instructions stay out of every kernel: some of their forms have
 # given wrong results on this hardware
@@ -55,7 +56,7 @@ def _wanted(sources: list[Path]) -> str:
     """What the built extension depends on, as a hash: its sources, compiler
     flags and architecture, and the torch and Python that load it."""
     h = hashlib.sha256()
-    for part in (_CXX_FLAGS, _HIP_FLAGS, os.environ["PYTORCH_ROCM_ARCH"],
+    for part in (_CXX_FLAGS, _HIP_FLAGS, os.environ.get(_ARCH, "gfx950"),
                  torch.__version__, torch.version.git_version,
                  torch.version.hip, sys.version_info[:2]):
         h.update(repr(part).encode() + b"\0")
@@ -87,7 +88,6 @@ def build_extension(verbose: bool = False, force: bool = False):
     global _C, _ERR
     if _C is not None and not force:
         return _C
-    os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
     build_dir = REPO_ROOT / "build" / "torch_ext"
     lib = build_dir / "baguanet_C.so"
     # written after a build: a library without it may be half written
@@ -123,6 +123,7 @@ def _compile(build_dir: Path, sources: list[Path], verbose: bool,
              force: bool):
     from torch.utils import cpp_extension
 
+    os.environ.setdefault(_ARCH, "gfx950")
     if force:
         for built in build_dir.glob("*.o"):
             built.unlink()

@@ -127,3 +127,18 @@ def test_directory_that_cannot_be_written_to(tree, monkeypatch):
 
     monkeypatch.setattr(type(tree.lib), "mkdir", refuse)
     assert tree.load() == "c.h" and tree.builds == 1
+
+
+def test_file_system_without_locks(tree, monkeypatch):
+    def refuse(file, how):
+        raise OSError("no locks available")
+
+    monkeypatch.setattr(ops.fcntl, "flock", refuse)
+    assert tree.load() == "c.h" and tree.load() == "c.h" and tree.builds == 1
+
+
+def test_loading_sets_no_architecture(tree, monkeypatch):
+    monkeypatch.delenv("PYTORCH_ROCM_ARCH", raising=False)
+    tree.load()
+    tree.load()
+    assert "PYTORCH_ROCM_ARCH" not in ops.os.environ and tree.builds == 1
