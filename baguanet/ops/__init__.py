@@ -69,15 +69,13 @@ def _wanted(sources: list[Path]) -> str:
 @contextlib.contextmanager
 def _locked(build_dir: Path, how: int):
     """The build directory's lock: shared to load, exclusive to build.  It ends
-    with its process, and a directory that cannot be written to needs none."""
-    try:
-        build_dir.mkdir(parents=True, exist_ok=True)
-        file = open(build_dir / "baguanet_C.lock", "a")
-    except OSError:
-        yield
-        return
-    with file:
-        fcntl.flock(file, how)
+    with its process.  A directory that cannot be written to needs none, and a
+    file system may have none."""
+    with contextlib.ExitStack() as stack:
+        with contextlib.suppress(OSError):
+            build_dir.mkdir(parents=True, exist_ok=True)
+            file = stack.enter_context(open(build_dir / "baguanet_C.lock", "a"))
+            fcntl.flock(file, how)
         yield
 
 
