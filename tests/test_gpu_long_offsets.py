@@ -161,3 +161,22 @@ def test_wgrad_result():
     for s in (slice(0, 300), slice(64_900, 65_300), slice(n - 300, n)):
         want = dy[:, s].t().float() @ x.float()
         assert torch.equal(dw[s].float(), want.to(BF).float())
+
+
+@pytest.mark.parametrize("per", ["element", "row"])
+def test_repeated_gate_rows(per):
+    """A gate that stands for three sequences: terms past 2^31, and their sums
+    as those of a few rows alone."""
+    from baguanet import ops
+
+    rows, dim = 88_000, 8200
+    x = _noise(3 * rows, dim).view(3, rows, dim)
+    gate = x[0, :, :dim if per == "element" else 1].clone().requires_grad_()
+    y, _ = ops.gated_residual_norm(x, x, gate)
+    (dg,) = torch.autograd.grad(y, gate, x)
+    assert dg.shape == gate.shape
+    for s in (slice(0, 9), slice(85_800, 85_810), slice(rows - 9, rows)):
+        few = gate.detach()[s].clone().requires_grad_()
+        ys, _ = ops.gated_residual_norm(x[:, s], x[:, s], few)
+        (want,) = torch.autograd.grad(ys, few, x[:, s])
+        assert torch.equal(y[:, s], ys) and torch.equal(dg[s], want)
