@@ -11,8 +11,9 @@
 //
 // These kernels are bound by HBM; four lanes hold a group, 8 values each, and
 // find its largest value with two lane exchanges.  16384 rows of 8192 bf16
-// pairs: silu forward 208 us (5.2 TB/s), backward 201 (5.4); 16384 rows of
-// 4096 bf16 are packed in 39 us (5.3).  A large copy moves 5.0 TB/s.
+// pairs: silu forward 213 us (5.1 TB/s), backward 197 (5.5); 16384 rows of 4096
+// bf16 are packed in 37 us (5.5) and unpacked in 30 (6.7), into fp32 in 88
+// (3.8).  A large copy moves 5.0 TB/s.
 #include <hip/hip_runtime.h>
 
 #include "act8_codes.h"

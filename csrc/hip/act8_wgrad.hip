@@ -15,10 +15,10 @@
 // own products.
 //
 // Bound by the matrix cores, fed from LDS: 16384 x 8192 x 4096 bf16 takes 850
-// to 920 us (1.2 to 1.3 PFLOP/s, as the clock allows), where the library's
+// to 930 us (1.2 to 1.3 PFLOP/s, as the clock allows), where the library's
 // product of the uncompressed operands takes 980; 4096^3 takes 110 (1.25
 // PFLOP/s; 117).  With few rows a tile's start and its way out weigh most: 256
-// x 4096 x 25088 fp32 takes 213 us for 0.16 TFLOP and 411 MB of dW.
+// x 4096 x 25088 fp32 takes 212 to 222 us for 0.16 TFLOP and 411 MB of dW.
 #include <hip/hip_runtime.h>
 
 #include <cmath>

@@ -11,11 +11,11 @@
 // tokens is summed in fp32 from its run of the sorted positions.  No atomics
 // touch a gradient.
 //
-// 65536 tokens, a table of 131072 x 4096 bf16: lookup 151 us (7.1 TB/s read
-// and written: rows that are asked for again come from a cache), gradient 368
-// us, of which the sort with the zeroing of dW (1.07 GB) beside it takes 175,
-// the sums 179 and the join of runs 14.  A large copy moves 5.0 TB/s, a fill
-// 6.8.
+// 65536 tokens, 18600 of them different and a tenth padding, a table of 131072 x
+// 4096 bf16: lookup 150 us (690 MB, each row read once: 4.6 TB/s), gradient 369
+// us (1.56 GB, 4.2 TB/s), of which the sort with the zeroing of dW (1.07 GB)
+// beside it takes 178, the sums 177 and the join of runs 14.  A large copy moves
+// 5.0 TB/s, a fill 6.8.
 #include <hip/hip_runtime.h>
 
 #include "device_types.h"
@@ -112,8 +112,13 @@ __device__ inline bool zero_part(const Zero& z) {
 // Few tokens: an element's place is the number of those before it in the
 // order, and these are counted directly.  64 elements to a workgroup, one to a
 // lane; its 16 waves count them against every 16th run of 64 others, which
-// pass through the lanes' registers: 8 us for 2048 tokens and 22 for 8192,
-// where the four launches of a radix sort take 17 and 19.
+// pass through the lanes' registers: 8 us for 2048 tokens and 21 for 8192,
+// where the four launches of a radix sort take 17 and 19.  The table is zeroed
+// beside this one launch, which starts less than four do.  Lookup and gradient
+// of 2048 and 8192 tokens in us, counted and by radix: 44, 52 and 68, 79 for
+// 50000 x 2048 bf16; 33, 45 and 45, 52 for 131072 x 512; 27, 32 and 51, 48 for
+// 20011 x 1001; 19, 20 and 36, 24 for 1000 x 64, which is small enough that
+// only the sort counts.
 constexpr int kRankBlock = 1024;
 constexpr int kRankWaves = kRankBlock / kWave;
 
