@@ -70,9 +70,14 @@ void check_not_recorded(const char* op) {
 
 // Kernels read a tensor's memory: it has to be there, and to hold the values
 // themselves.  Wrappers of other tensors and tensors that only stand for zeros
-// have none.
+// have none, and a storage may have been freed or cut under its tensor.
 bool has_memory(const Tensor& t) {
-  return t.numel() == 0 || t.storage().data() != nullptr;
+  if (t.numel() == 0) return true;
+  int64_t last = t.storage_offset();
+  for (int64_t d = 0; d < t.dim(); d++) last += (t.size(d) - 1) * t.stride(d);
+  const c10::Storage& s = t.storage();
+  return s.data() != nullptr &&
+         (size_t)(last + 1) * t.element_size() <= s.nbytes();
 }
 
 void check_plain(const Tensor& t, const char* op, const char* name) {
@@ -127,8 +132,9 @@ class OpNode : public torch::autograd::Node {
   // Only once t has been written: a hook may copy it here.
   void keep(size_t i, const Tensor& t) {
     saved_[i] = torch::autograd::SavedVariable(t, false);
-    if (saved_[i].has_hooks())
-      saved_as_[i] = {t.options(), t.sizes().vec(), t.is_contiguous()};
+    if (t.defined())
+      saved_as_[i] = {t.scalar_type(), t.device(), t.is_contiguous(),
+                      is_aligned(t), at::DimVector(t.sizes())};
   }
 
   void release_variables() override {
@@ -145,33 +151,37 @@ class OpNode : public torch::autograd::Node {
     std::array<Tensor, N> t;
     for (size_t i = 0; i < N; i++) {
       t[i] = saved_[i].unpack();
-      if (saved_[i].has_hooks()) t[i] = as_saved(op, t[i], saved_as_[i]);
+      if (t[i].defined()) t[i] = as_saved(op, t[i], saved_as_[i]);
     }
     return t;
   }
 
  private:
   struct Meta {
-    at::TensorOptions options;
-    std::vector<int64_t> sizes;
-    bool contiguous;
+    at::ScalarType type = at::kByte;
+    at::Device device = at::kCPU;
+    bool contiguous = false, aligned = false;
+    at::DimVector sizes;
   };
 
-  // What a hook gave back for a kept tensor: the kernels read it by the type,
-  // place and sizes that it had, and take rows and codes as aligned as torch's
-  // allocator makes them.
+  // A kept tensor as it was kept.  A hook may give another one back, and a
+  // parameter's data may have been exchanged (a module's half(), its move to
+  // another device) without counting as a change in place; but the kernels read
+  // it by the type, place and sizes that it had, weights and codes without gaps
+  // and codes in whole words.
   static Tensor as_saved(const char* op, const Tensor& t, const Meta& m) {
-    TORCH_CHECK(t.layout() == at::kStrided &&
-                    t.scalar_type() == m.options.dtype().toScalarType() &&
-                    t.device() == m.options.device() && t.sizes() == m.sizes,
-                op, ": a hook on kept tensors gave back ", t.scalar_type(), " ",
-                t.sizes(), " on ", t.device(), " for ",
-                m.options.dtype().toScalarType(), " ",
-                at::IntArrayRef(m.sizes), " on ", m.options.device());
+    TORCH_CHECK(t.layout() == at::kStrided && t.scalar_type() == m.type &&
+                    t.device() == m.device && t.sizes() == m.sizes,
+                op, ": a kept tensor has become ", t.scalar_type(), " ",
+                t.sizes(), " on ", t.device(), " from ", m.type, " ",
+                at::IntArrayRef(m.sizes), " on ", m.device);
     Tensor own = plain(t);
     if (m.contiguous) own = own.contiguous();
-    const bool aligned = ((uintptr_t)own.const_data_ptr() & 15) == 0;
-    return aligned || !m.contiguous ? own : own.clone();
+    return m.aligned && !is_aligned(own) ? own.clone() : own;
+  }
+
+  static bool is_aligned(const Tensor& t) {
+    return ((uintptr_t)t.const_data_ptr() & 15) == 0;
   }
 
   std::array<torch::autograd::SavedVariable, N> saved_;

@@ -413,7 +413,7 @@ def test_hook_that_gives_back_another_tensor(which, unpack):
     would read past its end."""
     f, leaves = _each_operator()[which]
     y = _through(f, leaves, unpack)
-    with pytest.raises(RuntimeError, match="hook on kept tensors"):
+    with pytest.raises(RuntimeError, match="kept tensor has become"):
         torch.autograd.grad(y.sum(), leaves, allow_unused=True)
 
 
@@ -466,3 +466,51 @@ def test_block_holds_its_codes_outputs_and_branch():
     kept = rows * (6 * dim + 8 + 33 / 32 * (dim + hidden + 2 * hidden))
     assert kept <= now <= kept + 16 * 512
     del out
+
+
+def test_kept_tensors_that_are_exchanged():
+    """Other data under a kept tensor, which is no change in place, and a
+    storage that was freed: refused, not read as what it was."""
+    from baguanet import ops
+
+    def norm():
+        x, o, gate, post, pre = (torch.randn(*s, device="cuda") for s in
+                                 ((6, 40), (6, 40), (40,), (40,), (40,)))
+        leaves = x, o, gate, post, pre
+        for t in (gate, post, pre):
+            t.requires_grad_()
+        return leaves, ops.gated_residual_norm(*leaves)[1]
+
+    def exchange(f):
+        def change(t):
+            t.data = f(t.data)
+        return change
+
+    changes = [exchange(lambda d: d.to(BF)), exchange(lambda d: d.cpu()),
+               exchange(lambda d: d[:1])]
+    for i in range(5):
+        for change in changes:
+            leaves, h = norm()
+            change(leaves[i])
+            # a gradient that no longer fits its leaf may be refused before
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(h.sum(), leaves[4 if i != 4 else 3])
+        leaves, h = norm()
+        size = leaves[i].untyped_storage().size()
+        leaves[i].untyped_storage().resize_(size // 2)
+        with pytest.raises(RuntimeError, match="no values of its own"):
+            torch.autograd.grad(h.sum(), leaves[4 if i != 4 else 3])
+    # the same values in another place are as good
+    leaves, h = norm()
+    want = torch.autograd.grad(h.sum(), leaves[2:], retain_graph=True)
+    for t in leaves:
+        t.data = t.data.clone()
+    got = torch.autograd.grad(h.sum(), leaves[2:])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for change in changes[:2]:
+        w = torch.randn(9, 40, device="cuda", requires_grad=True)
+        tok = torch.tensor([3, 1, 3], device="cuda")
+        y = ops.embedding(w, tok)
+        tok.data = tok.to(torch.int32) if change is changes[0] else tok.cpu()
+        with pytest.raises(RuntimeError, match="kept tensor has become"):
+            torch.autograd.grad(y.sum(), w)

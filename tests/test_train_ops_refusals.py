@@ -228,3 +228,20 @@ def test_table_too_large_for_its_gradient_refused(rows, cols):
                                        .requires_grad_(), TOK)):
         with pytest.raises(RuntimeError, match="must be on the GPU"):
             call()
+
+
+def test_freed_storage_refused():
+    for size in (0, 4 * 31):
+        x = torch.zeros(4, 8)
+        x.untyped_storage().resize_(size)
+        with pytest.raises(RuntimeError, match="x holds no values"):
+            ops.rms_norm(x)
+    x = torch.zeros(64)
+    for view in (x[32:].view(4, 8), x.as_strided((4, 8), (16, 1), 8),
+                 x[:8].expand(4, 8), x[63:].expand(4, 8)):
+        with pytest.raises(RuntimeError, match="must be on the GPU"):
+            ops.rms_norm(view)
+    view = x[32:].view(4, 8)
+    x.untyped_storage().resize_(4 * 63)
+    with pytest.raises(RuntimeError, match="x holds no values"):
+        ops.rms_norm(view)
